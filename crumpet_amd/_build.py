@@ -2,9 +2,9 @@
 
 * ``libcrumpet_hip.so``: the gfx950 HIP kernels and their C ABI
   (include/crumpet_hip.h), compiled by hipcc, one object per source.
-* ``_crumpet_ops.so``: the torch dispatcher binding (csrc/torch_binding.cpp),
-  compiled by g++ against the torch headers and linked to libcrumpet_hip.so
-  through an ``$ORIGIN`` rpath.
+* ``_crumpet_ops.so``: the torch dispatcher binding (csrc/torch_binding.cpp and
+  csrc/training_binding.cpp), compiled by g++ against the torch headers and
+  linked to libcrumpet_hip.so through an ``$ORIGIN`` rpath.
 
 Both land next to this file so that they travel with the source tree.  The
 HIP library records NEEDED ``libamdhip64.so.7``; once torch is imported the
@@ -37,7 +37,10 @@ HIP_SOURCES = [
     "attention_f16.hip", "attention_bf16.hip", "attention_f32.hip", "attention_d32.hip", "attention_wide.hip",
     "attention_chunk.hip",
     "window_linear.hip", "block_tail.hip",
+    "attention_train.hip", "attention_train_f16.hip", "attention_train_bf16.hip", "attention_train_f32.hip",
+    "bias_buckets.hip", "residual_norm.hip", "linear_8bit.hip",
 ]
+BINDING_SOURCES = ["torch_binding.cpp", "training_binding.cpp"]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",
@@ -99,12 +102,19 @@ def build_hip(verbose: bool = False, extra_flags: list[str] | None = None) -> Pa
 def build_binding(verbose: bool = False) -> Path:
     tinc, tlib = _torch_paths()
     tmp = OPS_LIB.with_suffix(".so.tmp")
-    cmd = [
-        "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+    BUILD_DIR.mkdir(exist_ok=True)
+    flags = [
+        "-O2", "-std=c++17", "-fPIC",
         "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
         f"-I{tinc}", f"-I{tinc / 'torch' / 'csrc' / 'api' / 'include'}",
         f"-I{ROCM / 'include'}", f"-I{INCLUDE}",
-        str(CSRC / "torch_binding.cpp"),
+    ]
+    objs = [BUILD_DIR / (src.rsplit(".", 1)[0] + ".o") for src in BINDING_SOURCES]
+    cmds = [["g++", *flags, "-c", str(CSRC / src), "-o", str(obj)] for src, obj in zip(BINDING_SOURCES, objs)]
+    with ThreadPoolExecutor(max_workers=len(cmds)) as pool:
+        list(pool.map(lambda c: _run(c, verbose), cmds))
+    cmd = [
+        "g++", "-shared", *map(str, objs),
         "-o", str(tmp),
         f"-L{PKG}", "-lcrumpet_hip",
         f"-L{tlib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip",

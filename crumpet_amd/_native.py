@@ -40,6 +40,18 @@ C_ABI_SYMBOLS = (
     "crumpet_rows_norm",
     "crumpet_merge_norm_3d",
     "crumpet_rows_linear",
+    "crumpet_bucket_segment",
+    "crumpet_bucket_bias",
+    "crumpet_bucket_bias_backward",
+    "crumpet_window_attention",
+    "crumpet_window_attention_workspace",
+    "crumpet_window_attention_backward",
+    "crumpet_residual_norm",
+    "crumpet_residual_norm_workspace",
+    "crumpet_residual_norm_backward",
+    "crumpet_linear_8bit",
+    "crumpet_linear_8bit_workspace",
+    "crumpet_linear_8bit_backward",
 )
 
 OP_NAMES = (
@@ -59,6 +71,16 @@ OP_NAMES = (
     "swin_mlp",
     "patch_merge_3d",
     "channel_norm",
+    "bucket_bias",
+    "bucket_bias_backward",
+    "window_attention",
+    "window_attention_forward",
+    "window_attention_backward",
+    "residual_norm",
+    "residual_norm_backward",
+    "linear_8bit",
+    "linear_8bit_forward",
+    "linear_8bit_backward",
 )
 
 _hip = None
@@ -123,12 +145,74 @@ def _channel_norm_fake(x, weight, bias, eps, dtype):
     return x.new_empty(x.shape, dtype=dtype)
 
 
+def _bucket_bias_fake(table, index, order, segments, firsts):
+    return table.new_empty((table.shape[1], *index.shape))
+
+
+def _bucket_bias_backward_fake(grad, order, segments, firsts, buckets):
+    return grad.new_empty((buckets, grad.shape[0]))
+
+
+def _window_attention_fake(qkv, bias, heads, mask, region, scale):
+    return qkv.new_empty((qkv.shape[0], qkv.shape[1], qkv.shape[2] // 3))
+
+
+def _window_attention_forward_fake(qkv, bias, heads, mask, region, scale):
+    out = _window_attention_fake(qkv, bias, heads, mask, region, scale)
+    rest = out.new_empty((0,) if qkv.dtype == torch.float32 else out.shape)
+    rows = qkv.new_empty((qkv.shape[0] * heads * qkv.shape[1],), dtype=torch.float32)
+    return out, rest, rows, torch.empty_like(rows)
+
+
+def _window_attention_backward_fake(grad, qkv, bias, heads, mask, region, scale, out, out_rest, row_max, row_inv,
+                                    want_bias):
+    return qkv.new_empty(qkv.shape), bias.new_empty(bias.shape if want_bias else (0,))
+
+
+def _residual_norm_fake(x, y, norm, post, post_weight, post_bias, gate, scale, weight, bias, eps):
+    return x.new_empty(x.shape), y.new_empty(y.shape)
+
+
+def _residual_norm_backward_fake(grad_sum, grad_out, x, y, norm, post, post_weight, post_bias, gate, scale, weight,
+                                 bias, eps, want):
+    params = (weight, bias, gate, post_weight, post_bias)
+    grads = [x.new_empty((0,), dtype=torch.float32) if p is None else p.new_empty(p.shape if want >> i & 1 else (0,))
+             for i, p in enumerate(params)]
+    return (x.new_empty(x.shape), y.new_empty(y.shape), *grads)
+
+
+def _linear_8bit_fake(x, weight, bias, activation):
+    return x.new_empty((*x.shape[:-1], weight.shape[0]))
+
+
+def _linear_8bit_forward_fake(x, weight, bias, activation):
+    rows, k = x.numel() // x.shape[-1], x.shape[-1]
+    codes = x.new_empty((rows, k), dtype=torch.int8)
+    return _linear_8bit_fake(x, weight, bias, activation), codes, codes.new_empty((rows, (k + 31) // 32))
+
+
+def _linear_8bit_backward_fake(grad, codes, exps, weight, activation, want_x, want_weight, want_bias):
+    return (grad.new_empty((*grad.shape[:-1], weight.shape[1]) if want_x else (0,)),
+            grad.new_empty(weight.shape if want_weight else (0,)),
+            grad.new_empty((weight.shape[0],) if want_bias else (0,)))
+
+
 _RETURNING_FAKES = {
     "window_msa_3d": _window_msa_fake,
     "window_permute_3d": _window_permute_fake,
     "swin_mlp": _swin_mlp_fake,
     "patch_merge_3d": _patch_merge_fake,
     "channel_norm": _channel_norm_fake,
+    "bucket_bias": _bucket_bias_fake,
+    "bucket_bias_backward": _bucket_bias_backward_fake,
+    "window_attention": _window_attention_fake,
+    "window_attention_forward": _window_attention_forward_fake,
+    "window_attention_backward": _window_attention_backward_fake,
+    "residual_norm": _residual_norm_fake,
+    "residual_norm_backward": _residual_norm_backward_fake,
+    "linear_8bit": _linear_8bit_fake,
+    "linear_8bit_forward": _linear_8bit_forward_fake,
+    "linear_8bit_backward": _linear_8bit_backward_fake,
 }
 
 

@@ -1,0 +1,172 @@
+// Window attention with gradients: argument checks, the choice of kernels and
+// the C ABI (kernels: attention_train_kernels.h).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "attention_train.h"
+#include "crumpet_hip.h"
+
+namespace crumpet {
+namespace train {
+namespace {
+
+constexpr int kThreads = 256;
+
+// out[i] = sum over the chunks of partial[chunk][i], in order
+__global__ void __launch_bounds__(kThreads)
+join_kernel(float* __restrict__ out, const float* __restrict__ partial, int64_t n, uint32_t chunks) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    if (i >= n) return;
+    float v = 0.0f;
+#pragma unroll 4
+    for (uint32_t c = 0; c < chunks; ++c) v += partial[c * n + i];
+    out[i] = v;
+}
+
+// Partial sums of dbias: enough that about 1024 workgroups share the windows,
+// within 256 MB.
+uint32_t bias_chunks(int64_t B, int64_t H, int64_t N) {
+    const int64_t blocks = H * ((N + 63) / 64) * ((N + 63) / 64);
+    const int64_t most = std::max<int64_t>(1, (int64_t(256) << 20) / (H * N * N * 4));
+    return static_cast<uint32_t>(std::max<int64_t>(1, std::min(std::min(B, most), (1024 + blocks - 1) / blocks)));
+}
+
+int64_t rounded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+int check(AttnArgs& a, int32_t dtype, int64_t B, int64_t H, int64_t N, int64_t D, const int64_t strides[2],
+          const float* bias, const void* mask, int32_t mask_dtype, int64_t mask_batch, int64_t mask_stride,
+          const int64_t* region, float scale, const char* what) {
+    if (dtype < 0 || dtype > 2 || (mask != nullptr && (mask_dtype < 0 || mask_dtype > 2)))
+        return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: unknown dtype code", what);
+    if (B < 0 || H < 0 || N < 0) return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: negative size", what);
+    if (D != 16 && D != 32 && D != 64 && D != 128)
+        return fail(CRUMPET_ERR_UNSUPPORTED, "%s: head_dim %lld is not 16, 32, 64 or 128", what, (long long)D);
+    if (N > 16384 || H > 4096 || B >= (int64_t(1) << 31))
+        return fail(CRUMPET_ERR_UNSUPPORTED, "%s: more than 16384 tokens, 4096 heads or 2^31 windows", what);
+    if (!launch_takes(static_cast<uint64_t>(B) * H * ((N + 15) / 16) + kNumXcd, kThreads) ||
+        !launch_takes((static_cast<uint64_t>(H) * N * N + kThreads - 1) / kThreads, kThreads))
+        return fail(CRUMPET_ERR_UNSUPPORTED, "%s: too many windows, heads or tokens for one launch", what);
+    if (B == 0 || H == 0 || N == 0) return CRUMPET_OK;
+    if (bias == nullptr) return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: null bias", what);
+    if (mask != nullptr && region != nullptr)
+        return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: a mask tensor and a shifted volume exclude each other", what);
+    const int64_t align = 16 / (dtype == CRUMPET_DTYPE_F32 ? 4 : 2);
+    if (strides[0] % align != 0 || strides[1] % align != 0)
+        return fail(CRUMPET_ERR_UNSUPPORTED, "%s: qkv rows must be 16-byte aligned", what);
+    a.sb = strides[0], a.st = strides[1], a.bias = bias, a.scale = scale;
+    a.B = static_cast<uint32_t>(B), a.H = static_cast<int32_t>(H), a.N = static_cast<int32_t>(N);
+    a.chunks = bias_chunks(B, H, N);
+    if (mask != nullptr) {
+        if (mask_batch < 1 || B % mask_batch != 0)
+            return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: the windows (%lld) must be a multiple of the masks (%lld)",
+                        what, (long long)B, (long long)mask_batch);
+        a.mode = kTensorMask, a.mask = mask, a.mask_dtype = mask_dtype;
+        a.mask_batch = static_cast<uint32_t>(mask_batch), a.mask_sb = mask_stride;
+    }
+    if (region != nullptr) {
+        const int64_t *volume = region, *ws = region + 3, *ss = region + 6;
+        int64_t nw[3];
+        for (int i = 0; i < 3; ++i) {
+            if (ws[i] < 1 || volume[i] < 1 || volume[i] % ws[i] != 0)
+                return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: the volume must be divisible by window_size", what);
+            if (ss[i] < 0 || ss[i] >= ws[i])
+                return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: shift_size must lie in [0, window_size)", what);
+            nw[i] = volume[i] / ws[i];
+            if (ws[i] > N || nw[i] > B) break;
+        }
+        if (ws[0] > N || ws[1] > N || ws[2] > N || ws[0] * ws[1] * ws[2] != N)
+            return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: N = %lld is not the window volume", what, (long long)N);
+        if (nw[0] > B || nw[1] > B || nw[2] > B || nw[0] * nw[1] > B || B % (nw[0] * nw[1] * nw[2]) != 0)
+            return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: the windows (%lld) must be a multiple of the volume's", what,
+                        (long long)B);
+        Region& r = a.region;
+        r.plane.init(static_cast<uint32_t>(ws[1] * ws[2]));
+        r.row.init(static_cast<uint32_t>(ws[2]));
+        r.grid_hw.init(static_cast<uint32_t>(nw[1] * nw[2]));
+        r.grid_w.init(static_cast<uint32_t>(nw[2]));
+        r.windows.init(static_cast<uint32_t>(nw[0] * nw[1] * nw[2]));
+        for (int i = 0; i < 3; ++i) {
+            r.from[i] = static_cast<int32_t>(ws[i] - ss[i]);
+            r.last[i] = ss[i] > 0 ? static_cast<int32_t>(nw[i] - 1) : -1;
+        }
+        if (ss[0] > 0 || ss[1] > 0 || ss[2] > 0) a.mode = kRegionMask;
+    }
+    return CRUMPET_OK;
+}
+
+bool misaligned(std::initializer_list<const void*> ptrs) {
+    for (const void* p : ptrs)
+        if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return true;
+    return false;
+}
+
+}  // namespace
+}  // namespace train
+}  // namespace crumpet
+
+using namespace crumpet;
+using namespace crumpet::train;
+
+extern "C" int crumpet_window_attention(void* out, void* out_rest, float* row_max, float* row_inv, const void* qkv,
+                                        const int64_t qkv_strides[2], int32_t dtype, int64_t B, int64_t heads,
+                                        int64_t N, int64_t head_dim, const float* bias, const void* mask,
+                                        int32_t mask_dtype, int64_t mask_batch, int64_t mask_stride,
+                                        const int64_t* region, float scale, void* stream) {
+    const char* what = "window_attention";
+    AttnArgs a = {};
+    const int st = train::check(a, dtype, B, heads, N, head_dim, qkv_strides, bias, mask, mask_dtype, mask_batch,
+                                mask_stride, region, scale, what);
+    if (st != CRUMPET_OK || B == 0 || heads == 0 || N == 0) return st;
+    if (out == nullptr || qkv == nullptr || (row_max == nullptr) != (row_inv == nullptr))
+        return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: null tensor", what);
+    if (misaligned({out, out_rest, qkv}))
+        return fail(CRUMPET_ERR_UNSUPPORTED, "%s: pointers must be 16-byte aligned", what);
+    a.out = out, a.out_lo = out_rest, a.row_max = row_max, a.row_inv = row_inv, a.qkv = qkv;
+    const int D = static_cast<int>(head_dim);
+    if (dtype == CRUMPET_DTYPE_F16) return attention_forward_f16(a, D, stream);
+    if (dtype == CRUMPET_DTYPE_BF16) return attention_forward_bf16(a, D, stream);
+    return attention_forward_f32(a, D, stream);
+}
+
+extern "C" int64_t crumpet_window_attention_workspace(int64_t B, int64_t heads, int64_t N) {
+    if (B < 0 || heads < 0 || N < 0 || B >= (int64_t(1) << 31) || heads > 4096 || N > 16384) return -1;
+    if (B == 0 || heads == 0 || N == 0) return 0;
+    return rounded(B * heads * N * 4) + bias_chunks(B, heads, N) * heads * N * N * 4;
+}
+
+extern "C" int crumpet_window_attention_backward(void* grad_qkv, float* grad_bias, const void* grad_out, const void* out,
+                                                 const void* out_rest, const float* row_max, const float* row_inv,
+                                                 const void* qkv, const int64_t qkv_strides[2], int32_t dtype,
+                                                 int64_t B, int64_t heads, int64_t N, int64_t head_dim,
+                                                 const float* bias, const void* mask, int32_t mask_dtype,
+                                                 int64_t mask_batch, int64_t mask_stride, const int64_t* region,
+                                                 float scale, void* workspace, void* stream) {
+    const char* what = "window_attention_backward";
+    AttnArgs a = {};
+    const int st = train::check(a, dtype, B, heads, N, head_dim, qkv_strides, bias, mask, mask_dtype, mask_batch,
+                                mask_stride, region, scale, what);
+    if (st != CRUMPET_OK || B == 0 || heads == 0 || N == 0) return st;
+    if (grad_qkv == nullptr || grad_out == nullptr || out == nullptr || row_max == nullptr || row_inv == nullptr ||
+        qkv == nullptr || workspace == nullptr || (dtype != CRUMPET_DTYPE_F32 && out_rest == nullptr))
+        return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: null tensor", what);
+    if (misaligned({grad_qkv, grad_out, out, out_rest, qkv, workspace}))
+        return fail(CRUMPET_ERR_UNSUPPORTED, "%s: pointers must be 16-byte aligned", what);
+    a.out = const_cast<void*>(out), a.out_lo = const_cast<void*>(out_rest), a.qkv = qkv;
+    a.row_max = const_cast<float*>(row_max), a.row_inv = const_cast<float*>(row_inv);
+    a.grad_out = grad_out, a.grad_qkv = grad_qkv;
+    char* ws = static_cast<char*>(workspace);
+    a.delta = reinterpret_cast<float*>(ws);
+    float* partial = reinterpret_cast<float*>(ws + rounded(B * heads * N * 4));
+    if (grad_bias != nullptr) a.grad_bias = a.chunks == 1 ? grad_bias : partial;
+    const int D = static_cast<int>(head_dim);
+    int rc;
+    if (dtype == CRUMPET_DTYPE_F16) rc = attention_backward_f16(a, D, stream);
+    else if (dtype == CRUMPET_DTYPE_BF16) rc = attention_backward_bf16(a, D, stream);
+    else rc = attention_backward_f32(a, D, stream);
+    if (rc != CRUMPET_OK || grad_bias == nullptr || a.chunks == 1) return rc;
+    const int64_t n = heads * N * N;
+    join_kernel<<<static_cast<uint32_t>((n + kThreads - 1) / kThreads), kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+        grad_bias, partial, n, a.chunks);
+    return check_launch(what);
+}

@@ -1,0 +1,163 @@
+// A learned bias by buckets (gfx950): bias[h, p] = table[index[p], h] over the
+// P pairs of query and key, and the table's gradient, the sum over the pairs of
+// each bucket.
+//
+// The gradient takes the pairs sorted by bucket (stable), cut into segments of
+// at most kSegment pairs that never cross a bucket: one wave per segment and
+// head sums its pairs in a fixed order, without atomics.  Where every bucket
+// fits one segment (the offsets of a window: 2,197 buckets of at most 343
+// pairs) that sum is the result; longer ones (few buckets over long sequences)
+// are partial sums, which a second kernel adds up.
+#include <hip/hip_runtime.h>
+
+#include "crumpet_common.h"
+#include "crumpet_hip.h"
+
+namespace crumpet {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kSegment = 2048;
+
+// Bits are copied, so one form per element size.  A workgroup writes 4 x 256
+// pairs of one head.  An index outside the table reads as 0.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+bucket_bias_kernel(T* __restrict__ out, const T* __restrict__ table, const int32_t* __restrict__ index, int64_t P,
+                   int32_t L, int32_t H) {
+    const int h = static_cast<int>(blockIdx.y);
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * (4 * kThreads) + threadIdx.x;
+    T* to = out + h * P;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t p = first + i * kThreads;
+        if (p >= P) break;
+        const int32_t l = index[p];
+        to[p] = static_cast<uint32_t>(l) < static_cast<uint32_t>(L) ? table[static_cast<int64_t>(l) * H + h] : T(0);
+    }
+}
+
+// segments [n, 2]: first pair (in sorted order) and one past the last
+template <typename T, typename To>
+__global__ void __launch_bounds__(kThreads)
+bucket_sum_kernel(To* __restrict__ out, const T* __restrict__ grad, const int32_t* __restrict__ order,
+                  const int32_t* __restrict__ segments, int64_t P, int32_t H, uint32_t n) {
+    const uint32_t unit = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+    const int h = static_cast<int>(blockIdx.y), lane = threadIdx.x & 63;
+    if (unit >= n) return;
+    const int64_t from = segments[2 * unit] < 0 ? 0 : segments[2 * unit];
+    const int64_t to = segments[2 * unit + 1] < P ? segments[2 * unit + 1] : P;
+    const T* g = grad + h * P;
+    float v = 0.0f;
+#pragma unroll 4
+    for (int64_t i = from + lane; i < to; i += 64) {
+        const uint32_t p = static_cast<uint32_t>(order[i]);
+        if (p < P) v += static_cast<float>(g[p]);
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+    if (lane == 0) out[static_cast<int64_t>(unit) * H + h] = static_cast<To>(v);
+}
+
+// firsts [L + 1]: each bucket's segments
+template <typename To>
+__global__ void __launch_bounds__(kThreads)
+bucket_join_kernel(To* __restrict__ out, const float* __restrict__ partial, const int32_t* __restrict__ firsts,
+                   int64_t L, int32_t H, uint32_t n) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (i >= L * H) return;
+    const int64_t l = i / H;
+    const int32_t h = static_cast<int32_t>(i % H);
+    const int64_t from = firsts[l] < 0 ? 0 : firsts[l], to = firsts[l + 1] < n ? firsts[l + 1] : n;
+    float v = 0.0f;
+    for (int64_t s = from + lane; s < to; s += 64) v += partial[s * H + h];
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+    if (lane == 0) out[i] = static_cast<To>(v);
+}
+
+int check(int32_t dtype, int64_t buckets, int64_t heads, int64_t pairs, const char* what) {
+    if (dtype < 0 || dtype > 2) return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: unknown dtype code", what);
+    if (buckets < 0 || heads < 0 || pairs < 0) return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: negative size", what);
+    if (buckets >= (int64_t(1) << 31) || pairs >= (int64_t(1) << 31) || heads > 65535)
+        return fail(CRUMPET_ERR_UNSUPPORTED, "%s: more than 2^31 buckets or pairs, or 65535 heads", what);
+    return CRUMPET_OK;
+}
+
+template <typename T>
+int backward(void* grad_table, const void* grad, int64_t L, int64_t H, int64_t P, const int32_t* order,
+             const int32_t* segments, int64_t n, const int32_t* firsts, float* partial, hipStream_t s) {
+    const dim3 grid(static_cast<uint32_t>((n + 3) / 4), static_cast<uint32_t>(H));
+    const T* g = static_cast<const T*>(grad);
+    if (firsts == nullptr) {  // one segment a bucket
+        bucket_sum_kernel<T, T><<<grid, kThreads, 0, s>>>(static_cast<T*>(grad_table), g, order, segments, P,
+                                                          static_cast<int32_t>(H), static_cast<uint32_t>(n));
+    } else {
+        if (n > 0)
+            bucket_sum_kernel<T, float><<<grid, kThreads, 0, s>>>(partial, g, order, segments, P,
+                                                                  static_cast<int32_t>(H), static_cast<uint32_t>(n));
+        bucket_join_kernel<T><<<static_cast<uint32_t>((L * H + 3) / 4), kThreads, 0, s>>>(
+            static_cast<T*>(grad_table), partial, firsts, L, static_cast<int32_t>(H), static_cast<uint32_t>(n));
+    }
+    return check_launch("bucket_bias_backward");
+}
+
+}  // namespace
+}  // namespace crumpet
+
+using namespace crumpet;
+
+extern "C" int64_t crumpet_bucket_segment(void) { return kSegment; }
+
+extern "C" int crumpet_bucket_bias(void* out, const void* table, int32_t dtype, const int32_t* index, int64_t buckets,
+                                   int64_t heads, int64_t pairs, void* stream) {
+    const int st = check(dtype, buckets, heads, pairs, "bucket_bias");
+    if (st != CRUMPET_OK || heads == 0 || pairs == 0) return st;
+    if (out == nullptr || table == nullptr || index == nullptr)
+        return fail(CRUMPET_ERR_INVALID_ARGUMENT, "bucket_bias: null tensor");
+    const dim3 grid(static_cast<uint32_t>((pairs + 4 * kThreads - 1) / (4 * kThreads)), static_cast<uint32_t>(heads));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == CRUMPET_DTYPE_F32)
+        bucket_bias_kernel<uint32_t><<<grid, kThreads, 0, s>>>(static_cast<uint32_t*>(out),
+                                                               static_cast<const uint32_t*>(table), index, pairs,
+                                                               static_cast<int32_t>(buckets),
+                                                               static_cast<int32_t>(heads));
+    else
+        bucket_bias_kernel<uint16_t><<<grid, kThreads, 0, s>>>(static_cast<uint16_t*>(out),
+                                                               static_cast<const uint16_t*>(table), index, pairs,
+                                                               static_cast<int32_t>(buckets),
+                                                               static_cast<int32_t>(heads));
+    return check_launch("bucket_bias");
+}
+
+extern "C" int crumpet_bucket_bias_backward(void* grad_table, const void* grad, int32_t dtype, int64_t buckets,
+                                            int64_t heads, int64_t pairs, const int32_t* order, const int32_t* segments,
+                                            int64_t segment_count, const int32_t* firsts, void* workspace,
+                                            void* stream) {
+    const char* what = "bucket_bias_backward";
+    const int st = check(dtype, buckets, heads, pairs, what);
+    if (st != CRUMPET_OK || heads == 0 || buckets == 0) return st;
+    if (grad_table == nullptr || segments == nullptr || (pairs > 0 && (grad == nullptr || order == nullptr)))
+        return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: null tensor", what);
+    if (segment_count < 0 || segment_count >= (int64_t(1) << 31) || (firsts == nullptr && segment_count != buckets))
+        return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: segments do not match the buckets", what);
+    if (firsts != nullptr && workspace == nullptr)
+        return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: null workspace", what);
+    if (!launch_takes(static_cast<uint64_t>(buckets) * heads / 4 + 1, kThreads) ||
+        !launch_takes(static_cast<uint64_t>(segment_count) / 4 + 1, kThreads))
+        return fail(CRUMPET_ERR_UNSUPPORTED, "%s: too many buckets or segments for one launch", what);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    float* partial = static_cast<float*>(workspace);
+    switch (dtype) {
+        case CRUMPET_DTYPE_F32:
+            return backward<float>(grad_table, grad, buckets, heads, pairs, order, segments, segment_count, firsts,
+                                   partial, s);
+        case CRUMPET_DTYPE_F16:
+            return backward<_Float16>(grad_table, grad, buckets, heads, pairs, order, segments, segment_count, firsts,
+                                      partial, s);
+        default:
+            return backward<__bf16>(grad_table, grad, buckets, heads, pairs, order, segments, segment_count, firsts,
+                                    partial, s);
+    }
+}

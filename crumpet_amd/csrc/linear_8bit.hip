@@ -1,0 +1,476 @@
+// A linear layer whose input is kept in 8 bits for the backward pass (gfx950):
+//   y = act(x) W^T + b,   dx = (dy W) act'(x^),   dW = dy^T act(x^),   db = sum dy
+// with act the identity or the exact GELU and x^ the 8-bit copy of x: for every
+// row and 32 columns whole numbers up to 127 times 2^e, e the least integer
+// >= -126 with 127 2^e >= the group's largest magnitude.  A power of two makes
+// both directions exact: the copy is x rounded to a multiple of 2^e, nothing
+// else, and an exponent is one byte.  A group with an infinity or NaN is kept
+// as NaN (exponent byte -128).
+//
+// Kept are 33/32 bytes a value instead of 2 for x and 2 more for act(x).
+//
+// Products are v_mfma_f32_16x16x32, fp32 accumulation, one rounding at the
+// end; act(x) and act(x^) are rounded to the input type once, as operands.
+// Weights are the A operand, rows of x the B operand, so a lane ends with 4
+// neighbouring output features of one row and x passes from memory straight
+// into B fragments: a 32-deep step is one quantisation group, spread over the
+// 4 lane groups.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "crumpet_common.h"
+#include "crumpet_hip.h"
+#include "train_mma.h"
+
+namespace crumpet {
+namespace train {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kGroup = 32;
+constexpr int kNaN = -128;  // exponent byte of a group that is not finite
+
+typedef int8_t i8x4 __attribute__((ext_vector_type(4)));
+typedef int8_t i8x8 __attribute__((ext_vector_type(8)));
+typedef int8_t i8x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ float power_of_two(int e) {
+    return e == kNaN ? __builtin_nanf("") : __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+
+// The normal distribution Phi(x) = erfc(-x / sqrt 2) / 2 and x times its
+// density.  erfc by formula 7.1.26 of Abramowitz & Stegun, Handbook of
+// Mathematical Functions (|error| <= 1.5e-7, far below a 16-bit result's
+// rounding); the negative side uses erfc itself, so nothing cancels.
+struct Normal {
+    float phi, x_density;
+    __device__ __forceinline__ explicit Normal(float x) {
+        const float z = fabsf(x) * 0.70710678f;
+        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, z, 1.0f));
+        float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+        p = __builtin_fmaf(p, t, 1.421413741f);
+        p = __builtin_fmaf(p, t, -0.284496736f);
+        p = __builtin_fmaf(p, t, 0.254829592f);
+        const float bell = __builtin_amdgcn_exp2f(z * z * -kLog2e);
+        const float half_erfc = 0.5f * p * t * bell;
+        phi = x > 0.0f ? 1.0f - half_erfc : half_erfc;
+        x_density = x * bell * 0.39894228f;
+    }
+};
+template <bool kGelu>
+__device__ __forceinline__ float act(float x) {
+    if constexpr (kGelu) return x * Normal(x).phi;
+    return x;
+}
+template <bool kGelu>
+__device__ __forceinline__ float act_grad(float x) {
+    if constexpr (kGelu) {
+        const Normal n(x);
+        return n.phi + n.x_density;
+    }
+    return 1.0f;
+}
+
+// Codes of 8 of a group's 32 values (the other lanes of the row hold the
+// rest), and the group's exponent.  Magnitudes compare as their bits, NaN
+// above everything.
+template <typename T>
+__device__ __forceinline__ i8x8 quantise(typename Mma<T>::x8 v, int& e) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t bits = __float_as_uint(static_cast<float>(v[i])) & 0x7fffffffu;
+        top = top > bits ? top : bits;
+    }
+#pragma unroll
+    for (int m = 16; m <= 32; m <<= 1) {
+        const uint32_t other = __shfl_xor(top, m);
+        top = top > other ? top : other;
+    }
+    // top = 1.f 2^k; 127 = 1.984375 2^6
+    const int k = static_cast<int>(top >> 23) - 127;
+    e = k - ((top & 0x7fffffu) > 0x7e0000u ? 5 : 6);
+    e = e < -126 ? -126 : e;
+    i8x8 codes = {};
+    if (top >= 0x7f800000u) {
+        e = kNaN;
+        return codes;
+    }
+    const float up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) codes[i] = static_cast<int8_t>(__builtin_rintf(static_cast<float>(v[i]) * up));
+    return codes;
+}
+
+struct RowsArgs {
+    const void* x;        // [rows, K]
+    const void* w;        // [n_out, K]
+    const void* b;        // [n_out] or null
+    void* y;              // [rows, n_out]
+    int8_t* codes;        // forward: [rows, K] or null; backward: [rows, n_out], read
+    int8_t* exps;         // [rows, ceil(columns / 32)]
+    int64_t rows;
+    int32_t K, n_out;
+};
+
+// y = f(x) w^T.  Forward: f = act, the bias added, codes written by the first
+// column block.  Backward (x = dy, w = W^T): y times act' of the codes at y's
+// place.  A wave owns 32 rows, a workgroup 128 rows and 16 NT columns.
+template <typename T, int NT, bool kGelu, bool kForward>
+__global__ void __launch_bounds__(kThreads) linear_8bit_rows_kernel(const RowsArgs a, uint32_t row_blocks, uint32_t blocks) {
+    typedef typename Mma<T>::x8 X8;
+    uint32_t id;
+    if (!xcd_chunk(blockIdx.x, gridDim.x, row_blocks * blocks, id)) return;
+    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    const int n0 = static_cast<int>(id % blocks) * 16 * NT;
+    const int64_t row0 = static_cast<int64_t>(id / blocks) * 128 + (threadIdx.x >> 6) * 32 + col;
+    const int groups = (a.K + kGroup - 1) / kGroup;
+    const bool keep = kForward && n0 == 0 && a.codes != nullptr;
+    const T* xr[2];
+    int64_t row[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        row[r] = row0 + 16 * r;
+        xr[r] = static_cast<const T*>(a.x) + (row[r] < a.rows ? row[r] : a.rows - 1) * a.K;
+    }
+    const T* wr[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int f = n0 + 16 * n + col;
+        wr[n] = static_cast<const T*>(a.w) + static_cast<int64_t>(f < a.n_out ? f : a.n_out - 1) * a.K;
+    }
+    f32x4 acc[NT][2] = {};
+    for (int k0 = 0; k0 < a.K; k0 += kGroup) {
+        const int k = k0 + 8 * g;
+        const bool in = k < a.K;  // K is a multiple of 16: a last half step
+        X8 xv[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            xv[r] = X8{};
+            if (in) xv[r] = *reinterpret_cast<const X8*>(xr[r] + k);
+        }
+        X8 wv[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            wv[n] = X8{};
+            if (in) wv[n] = *reinterpret_cast<const X8*>(wr[n] + k);
+        }
+        if constexpr (kForward) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                if (keep) {
+                    int e;
+                    const i8x8 codes = quantise<T>(xv[r], e);
+                    if (row[r] < a.rows) {
+                        if (in) *reinterpret_cast<i8x8*>(a.codes + row[r] * a.K + k) = codes;
+                        if (g == 0) a.exps[row[r] * groups + k0 / kGroup] = static_cast<int8_t>(e);
+                    }
+                }
+                if constexpr (kGelu) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) xv[r][i] = static_cast<T>(act<true>(static_cast<float>(xv[r][i])));
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) acc[n][r] = Mma<T>::mma32(wv[n], xv[r], acc[n][r]);
+        }
+    }
+    const int out_groups = (a.n_out + kGroup - 1) / kGroup;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int f = n0 + 16 * n + 4 * g;
+        if (f >= a.n_out) continue;
+        f32x4 bias = {};
+        if (kForward && a.b != nullptr) bias = wide4<T>(load4<T>(static_cast<const T*>(a.b) + f));
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            if (row[r] >= a.rows) continue;
+            f32x4 v = acc[n][r];
+            if constexpr (kForward) {
+                v += bias;
+            } else if constexpr (kGelu) {
+                const i8x4 c = *reinterpret_cast<const i8x4*>(a.codes + row[r] * a.n_out + f);
+                const float step = power_of_two(a.exps[row[r] * out_groups + f / kGroup]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] *= act_grad<true>(static_cast<float>(c[i]) * step);
+            }
+            *reinterpret_cast<typename Mma<T>::x4*>(static_cast<T*>(a.y) + row[r] * a.n_out + f) = round4<T>(v);
+        }
+    }
+}
+
+// out [K, n] = in [n, K]; 32 x 32 tiles through LDS.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) transpose_kernel(T* __restrict__ out, const T* __restrict__ in, int32_t n, int32_t K) {
+    __shared__ T tile[32][33];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const int k0 = blockIdx.x * 32, n0 = blockIdx.y * 32;
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+        if (n0 + y + i < n && k0 + x < K) tile[y + i][x] = in[static_cast<int64_t>(n0 + y + i) * K + k0 + x];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+        if (k0 + y + i < K && n0 + x < n) out[static_cast<int64_t>(k0 + y + i) * n + n0 + x] = tile[x][y + i];
+}
+
+struct WeightArgs {
+    const void* dy;          // [rows, n_out]
+    const int8_t* codes;     // [rows, K]
+    const int8_t* exps;
+    float* partial;          // [chunks, n_out K + n_out]
+    int64_t rows, per;       // rows of a chunk
+    int32_t K, n_out;
+    uint32_t kblocks, nblocks;
+};
+
+// A chunk of rows' share of a 64 x 128 tile of dW = dy^T act(x^), and of db.
+// Both operands are read along the rows, so they pass through LDS, row-major,
+// and come back by transpose reads; the depth's order is the same permutation
+// on both sides.  The codes become act(x^) on their way into LDS, once for
+// each value and column block.
+template <typename T, bool kGelu>
+__global__ void __launch_bounds__(kThreads) linear_8bit_weight_kernel(const WeightArgs a) {
+    typedef typename Mma<T>::x4 X4;
+    typedef typename Mma<T>::x8 X8;
+    constexpr int kRows = 64, kN = 64, kK = 128, kLdN = kN + 8, kLdK = kK + 8;
+    __shared__ __attribute__((aligned(16))) T dy_lds[kRows * kLdN];
+    __shared__ __attribute__((aligned(16))) T x_lds[kRows * kLdK];
+    uint32_t id = blockIdx.x;
+    const uint32_t kb = id % a.kblocks;
+    id /= a.kblocks;
+    const int n0 = static_cast<int>(id % a.nblocks) * kN, k0 = static_cast<int>(kb) * kK;
+    const int64_t chunk = id / a.nblocks;
+    const int64_t begin = chunk * a.per, end = std::min<int64_t>(a.rows, begin + a.per);
+    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
+    const int groups = (a.K + kGroup - 1) / kGroup;
+    const bool sum_dy = kb == 0 && wave == 0;
+    f32x4 acc[4][2] = {}, db[4] = {};
+    X8 ones;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ones[i] = static_cast<T>(1.0f);
+    for (int64_t r0 = begin; r0 < end; r0 += kRows) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int p = threadIdx.x + i * kThreads, r = p >> 3, c = (p & 7) * 8;
+            X8 v = {};
+            if (r0 + r < end && n0 + c < a.n_out)
+                v = *reinterpret_cast<const X8*>(static_cast<const T*>(a.dy) + (r0 + r) * a.n_out + n0 + c);
+            *reinterpret_cast<X8*>(dy_lds + r * kLdN + c) = v;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int p = threadIdx.x + i * kThreads, r = p >> 3, c = (p & 7) * 16;
+            X8 v[2] = {};
+            if (r0 + r < end && k0 + c < a.K) {
+                const i8x16 codes = *reinterpret_cast<const i8x16*>(a.codes + (r0 + r) * a.K + k0 + c);
+                const float step = power_of_two(a.exps[(r0 + r) * groups + (k0 + c) / kGroup]);
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    v[e >> 3][e & 7] = static_cast<T>(act<kGelu>(static_cast<float>(codes[e]) * step));
+            }
+            *reinterpret_cast<X8*>(x_lds + r * kLdK + c) = v[0];
+            *reinterpret_cast<X8*>(x_lds + r * kLdK + c + 8) = v[1];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int s = 0; s < kRows; s += 32) {
+            X8 av[4], bv[2];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const X4 lo = load_transposed<T>(dy_lds, kLdN, s, 16 * n, col, g);
+                const X4 hi = load_transposed<T>(dy_lds, kLdN, s + 16, 16 * n, col, g);
+                av[n] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int c = 32 * wave + 16 * t;
+                const X4 lo = load_transposed<T>(x_lds, kLdK, s, c, col, g);
+                const X4 hi = load_transposed<T>(x_lds, kLdK, s + 16, c, col, g);
+                bv[t] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                if (sum_dy) db[n] = Mma<T>::mma32(av[n], ones, db[n]);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) acc[n][t] = Mma<T>::mma32(av[n], bv[t], acc[n][t]);
+            }
+        }
+    }
+    float* to = a.partial + chunk * (static_cast<int64_t>(a.n_out) * a.K + a.n_out);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int f = n0 + 16 * n + 4 * g + r;
+            if (f >= a.n_out) continue;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int k = k0 + 32 * wave + 16 * t + col;
+                if (k < a.K) to[static_cast<int64_t>(f) * a.K + k] = acc[n][t][r];
+            }
+            if (sum_dy && col == 0) to[static_cast<int64_t>(a.n_out) * a.K + f] = db[n][r];
+        }
+    }
+}
+
+// Chunks added in order; the first `weights` sums go to dw, the rest to db.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) linear_8bit_join_kernel(T* dw, T* db, const float* __restrict__ partial,
+                                                                   int64_t weights, int64_t all, int64_t chunks) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    if (i >= all) return;
+    float v = 0.0f;
+#pragma unroll 8
+    for (int64_t c = 0; c < chunks; ++c) v += partial[c * all + i];
+    if (i < weights) {
+        if (dw != nullptr) dw[i] = static_cast<T>(v);
+    } else if (db != nullptr) {
+        db[i - weights] = static_cast<T>(v);
+    }
+}
+
+template <typename T, bool kGelu, bool kForward>
+int rows_product(const RowsArgs& a, hipStream_t s) {
+    const int tiles = a.n_out / 16;
+    const uint32_t row_blocks = static_cast<uint32_t>((a.rows + 127) / 128);
+    // the fewest column blocks of at most 8 tiles, evenly cut
+    const int blocks = (tiles + 7) / 8, nt = (tiles + blocks - 1) / blocks;
+    const uint32_t grid = xcd_launch_count(row_blocks * static_cast<uint32_t>(blocks));
+#define CRUMPET_ROWS(NT)                                                                                          \
+    case NT:                                                                                                      \
+        linear_8bit_rows_kernel<T, NT, kGelu, kForward><<<grid, kThreads, 0, s>>>(a, row_blocks,                  \
+                                                                                  static_cast<uint32_t>(blocks)); \
+        break;
+    switch (nt) {
+        CRUMPET_ROWS(1) CRUMPET_ROWS(2) CRUMPET_ROWS(3) CRUMPET_ROWS(4) CRUMPET_ROWS(5) CRUMPET_ROWS(6)
+        CRUMPET_ROWS(7) CRUMPET_ROWS(8)
+    }
+#undef CRUMPET_ROWS
+    return check_launch("linear_8bit");
+}
+
+struct Split {
+    uint32_t kblocks, nblocks;
+    int64_t chunks, per;
+};
+Split split_rows(int64_t rows, int64_t K, int64_t n_out) {
+    Split p;
+    p.kblocks = static_cast<uint32_t>((K + 127) / 128);
+    p.nblocks = static_cast<uint32_t>((n_out + 63) / 64);
+    // about 1024 workgroups, none with fewer than 256 rows
+    const int64_t want = std::max<int64_t>(1, 1024 / (static_cast<int64_t>(p.kblocks) * p.nblocks));
+    const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>(want, (rows + 255) / 256));
+    p.per = ((rows + chunks - 1) / chunks + 63) / 64 * 64;
+    p.chunks = std::max<int64_t>(1, (rows + p.per - 1) / p.per);
+    return p;
+}
+
+int check(int32_t dtype, int64_t rows, int64_t K, int64_t n_out, int32_t activation, const char* what) {
+    if (dtype != CRUMPET_DTYPE_F16 && dtype != CRUMPET_DTYPE_BF16)
+        return fail(dtype == CRUMPET_DTYPE_F32 ? CRUMPET_ERR_UNSUPPORTED : CRUMPET_ERR_INVALID_ARGUMENT,
+                    "%s: dtype must be float16 or bfloat16", what);
+    if (rows < 0 || K < 0 || n_out < 0) return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: negative size", what);
+    if (activation != 0 && activation != 1)
+        return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: activation is 0 (none) or 1 (gelu)", what);
+    if (K < 16 || n_out < 16 || K % 16 != 0 || n_out % 16 != 0 || K > 65536 || n_out > 65536)
+        return fail(CRUMPET_ERR_UNSUPPORTED, "%s: features in (%lld) and out (%lld) must be multiples of 16 up to 65536",
+                    what, (long long)K, (long long)n_out);
+    const uint64_t row_blocks = (static_cast<uint64_t>(rows) + 127) / 128;
+    if (!launch_takes(row_blocks * ((std::max(K, n_out) / 16 + 7) / 8) + kNumXcd, kThreads))
+        return fail(CRUMPET_ERR_UNSUPPORTED, "%s: too many rows for one launch", what);
+    return CRUMPET_OK;
+}
+
+bool misaligned(std::initializer_list<const void*> ptrs) {
+    for (const void* p : ptrs)
+        if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return true;
+    return false;
+}
+
+template <typename T>
+int backward(void* dx, void* dw, void* db, const void* dy, const int8_t* codes, const int8_t* exps, int64_t rows,
+             int64_t K, int64_t n_out, const void* w, int32_t activation, char* workspace, hipStream_t s) {
+    const int32_t k = static_cast<int32_t>(K), n = static_cast<int32_t>(n_out);
+    if (dx != nullptr) {
+        T* wt = reinterpret_cast<T*>(workspace);
+        transpose_kernel<T><<<dim3((k + 31) / 32, (n + 31) / 32), kThreads, 0, s>>>(wt, static_cast<const T*>(w), n, k);
+        RowsArgs a = {};
+        a.x = dy, a.w = wt, a.y = dx, a.rows = rows, a.K = n, a.n_out = k;
+        a.codes = const_cast<int8_t*>(codes), a.exps = const_cast<int8_t*>(exps);
+        const int rc = activation ? rows_product<T, true, false>(a, s) : rows_product<T, false, false>(a, s);
+        if (rc != CRUMPET_OK) return rc;
+    }
+    if (dw == nullptr && db == nullptr) return CRUMPET_OK;
+    const Split p = split_rows(rows, K, n_out);
+    WeightArgs a = {};
+    a.dy = dy, a.codes = codes, a.exps = exps, a.rows = rows, a.per = p.per, a.K = k, a.n_out = n;
+    a.partial = reinterpret_cast<float*>(workspace + (K * n_out * 2 + 255) / 256 * 256);
+    a.kblocks = p.kblocks, a.nblocks = p.nblocks;
+    const uint32_t grid = static_cast<uint32_t>(p.chunks) * p.kblocks * p.nblocks;
+    if (activation)
+        linear_8bit_weight_kernel<T, true><<<grid, kThreads, 0, s>>>(a);
+    else
+        linear_8bit_weight_kernel<T, false><<<grid, kThreads, 0, s>>>(a);
+    const int64_t all = n_out * K + n_out;
+    linear_8bit_join_kernel<T><<<static_cast<uint32_t>((all + kThreads - 1) / kThreads), kThreads, 0, s>>>(
+        static_cast<T*>(dw), static_cast<T*>(db), a.partial, n_out * K, all, p.chunks);
+    return check_launch("linear_8bit_backward");
+}
+
+}  // namespace
+}  // namespace train
+}  // namespace crumpet
+
+using namespace crumpet;
+using namespace crumpet::train;
+
+extern "C" int crumpet_linear_8bit(void* y, int8_t* codes, int8_t* exponents, const void* x, int32_t dtype,
+                                   int64_t rows, int64_t K, const void* weight, const void* bias, int64_t n_out,
+                                   int32_t activation, void* stream) {
+    const char* what = "linear_8bit";
+    const int st = train::check(dtype, rows, K, n_out, activation, what);
+    if (st != CRUMPET_OK || rows == 0) return st;
+    if (y == nullptr || x == nullptr || weight == nullptr || (codes == nullptr) != (exponents == nullptr))
+        return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: null tensor", what);
+    if (train::misaligned({y, codes, x, weight, bias}))
+        return fail(CRUMPET_ERR_UNSUPPORTED, "%s: pointers must be 16-byte aligned", what);
+    RowsArgs a = {};
+    a.x = x, a.w = weight, a.b = bias, a.y = y, a.codes = codes, a.exps = exponents;
+    a.rows = rows, a.K = static_cast<int32_t>(K), a.n_out = static_cast<int32_t>(n_out);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == CRUMPET_DTYPE_F16)
+        return activation ? rows_product<_Float16, true, true>(a, s) : rows_product<_Float16, false, true>(a, s);
+    return activation ? rows_product<__bf16, true, true>(a, s) : rows_product<__bf16, false, true>(a, s);
+}
+
+extern "C" int64_t crumpet_linear_8bit_workspace(int64_t rows, int64_t K, int64_t n_out) {
+    if (train::check(CRUMPET_DTYPE_F16, rows, K, n_out, 0, "linear_8bit_workspace") != CRUMPET_OK) return -1;
+    if (rows == 0) return 0;
+    return (K * n_out * 2 + 255) / 256 * 256 + split_rows(rows, K, n_out).chunks * (n_out * K + n_out) * 4;
+}
+
+extern "C" int crumpet_linear_8bit_backward(void* grad_x, void* grad_weight, void* grad_bias, const void* grad_y,
+                                            int32_t dtype, const int8_t* codes, const int8_t* exponents, int64_t rows,
+                                            int64_t K, const void* weight, int64_t n_out, int32_t activation,
+                                            void* workspace, void* stream) {
+    const char* what = "linear_8bit_backward";
+    const int st = train::check(dtype, rows, K, n_out, activation, what);
+    if (st != CRUMPET_OK || rows == 0) return st;
+    if (grad_y == nullptr || codes == nullptr || exponents == nullptr || weight == nullptr || workspace == nullptr)
+        return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: null tensor", what);
+    if (train::misaligned({grad_x, grad_y, codes, weight, workspace}))
+        return fail(CRUMPET_ERR_UNSUPPORTED, "%s: pointers must be 16-byte aligned", what);
+    char* ws = static_cast<char*>(workspace);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == CRUMPET_DTYPE_F16)
+        return train::backward<_Float16>(grad_x, grad_weight, grad_bias, grad_y, codes, exponents, rows, K, n_out,
+                                         weight, activation, ws, s);
+    return train::backward<__bf16>(grad_x, grad_weight, grad_bias, grad_y, codes, exponents, rows, K, n_out, weight,
+                                   activation, ws, s);
+}

@@ -1,0 +1,465 @@
+// The residual sum of a block's branch with the norms around it (gfx950), over
+// rows of C channels in S samples:
+//   y' = post ? norm(y) w_p + b_p : y
+//   x1 = x + k[sample] gate y',   h = norm(x1) w + b
+// with norm a LayerNorm or an RMS norm, and its gradients.
+//
+// Everything is bound by HBM: one pass each way, a row in the registers of a
+// group of lanes (8 to 64 lanes of a wave, or the workgroup), 8 channels a
+// lane and load where C allows.  The backward pass reads x and y again and
+// computes x1 and both norms anew, so that nothing but the inputs is kept for
+// it and no rounded sum enters the gradients: x1 and h come from the same fp32
+// values, each rounded once.  Sums over channels and rows are fp32, in a fixed
+// order: each workgroup sums its rows' parameter gradients in registers and
+// writes one row of partial sums, which a second kernel adds up.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "crumpet_common.h"
+#include "crumpet_hip.h"
+
+namespace crumpet {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kSums = 5;  // w, b, gate, w_p, b_p
+
+struct NormArgs {
+    const void *x, *y;
+    const float *pw, *pb, *gate, *scale, *w, *b;  // each may be null but w
+    void *sum, *out;                              // forward
+    const void *gsum, *gout;                      // backward; gsum or gout may be null
+    void *gx, *gy;
+    float* partial;                               // [S * chunks, kSums, C]
+    uint32_t S, T, chunks;                        // samples, rows of a sample, workgroups of a sample
+    int32_t C;
+    int32_t gate_stride;                          // 0 or C
+    int32_t post, rms;
+    float eps, post_eps;
+};
+
+template <typename T, int E>
+__device__ __forceinline__ void load_row(const T* p, float* v) {
+    if constexpr (E == 1) {
+        v[0] = static_cast<float>(p[0]);
+    } else {
+        typedef T TE __attribute__((ext_vector_type(E)));
+        const TE t = *reinterpret_cast<const TE*>(p);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = static_cast<float>(t[e]);
+    }
+}
+template <typename T, int E>
+__device__ __forceinline__ void store_row(T* p, const float* v) {
+    if constexpr (E == 1) {
+        p[0] = static_cast<T>(v[0]);
+    } else {
+        typedef T TE __attribute__((ext_vector_type(E)));
+        TE t;
+#pragma unroll
+        for (int e = 0; e < E; ++e) t[e] = static_cast<T>(v[e]);
+        *reinterpret_cast<TE*>(p) = t;
+    }
+}
+
+// Sum over the G lanes of a row; G = 256 takes a round through LDS.
+template <int G>
+__device__ __forceinline__ float row_sum(float v, float* lds) {
+#pragma unroll
+    for (int m = 1; m < (G < 64 ? G : 64); m <<= 1) v += __shfl_xor(v, m);
+    if constexpr (G == 256) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = lds[0] + lds[1] + lds[2] + lds[3];
+    }
+    return v;
+}
+
+// One lane's share of a row: NV vectors of E channels, vector i at channel
+// (i G + lane) E.
+template <int E, int NV, int G>
+struct Lane {
+    int at[NV];
+    bool in[NV];
+    __device__ __forceinline__ explicit Lane(int C) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            at[i] = (i * G + static_cast<int>(threadIdx.x) % G) * E;
+            in[i] = at[i] < C;  // C is a multiple of E
+        }
+    }
+    template <typename T>
+    __device__ __forceinline__ void load(const T* row, float* v, float dflt = 0.0f) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (row != nullptr && in[i]) {
+                load_row<T, E>(row + at[i], v + i * E);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[i * E + e] = dflt;
+            }
+        }
+    }
+    template <typename T>
+    __device__ __forceinline__ void store(T* row, const float* v) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (in[i]) store_row<T, E>(row + at[i], v + i * E);
+    }
+    // v -> (v - mean) r, or v r without the mean; returns r = 1 / deviation
+    __device__ __forceinline__ float normalise(float* v, int C, bool rms, float eps, float* lds) const {
+        const float per = 1.0f / static_cast<float>(C);
+        float mean = 0.0f;
+        if (!rms) {
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NV * E; ++i) s += v[i];
+            mean = row_sum<G>(s, lds) * per;
+        }
+        float q = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                float& t = v[i * E + e];
+                t = in[i] ? t - mean : 0.0f;
+                q = __builtin_fmaf(t, t, q);
+            }
+        }
+        const float r = 1.0f / sqrtf(row_sum<G>(q, lds) * per + eps);
+#pragma unroll
+        for (int i = 0; i < NV * E; ++i) v[i] *= r;
+        return r;
+    }
+    // g (gradient of the normed values n) -> gradient of the values; 0 past the row
+    __device__ __forceinline__ void normalise_grad(float* g, const float* n, float r, int C, bool rms, float* lds) const {
+        const float per = 1.0f / static_cast<float>(C);
+        float a = 0.0f, c = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV * E; ++i) {
+            a += g[i];
+            c = __builtin_fmaf(g[i], n[i], c);
+        }
+        a = rms ? 0.0f : row_sum<G>(a, lds) * per;
+        c = row_sum<G>(c, lds) * per;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int e = i * E; e < (i + 1) * E; ++e) g[e] = in[i] ? r * (g[e] - a - n[e] * c) : 0.0f;
+        }
+    }
+};
+
+template <typename Tx, typename Ty, int E, int NV, int G>
+__global__ void __launch_bounds__(kThreads) residual_norm_kernel(const NormArgs a) {
+    __shared__ float lds[4];
+    constexpr int kRows = kThreads / G, kN = NV * E;
+    const Lane<E, NV, G> lane(a.C);
+    const uint32_t sample = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+    const float k = a.scale != nullptr ? a.scale[sample] : 1.0f;
+    float w[kN], b[kN], kg[kN];
+    lane.load(a.w, w, 1.0f);
+    lane.load(a.b, b);
+    lane.load(a.gate != nullptr ? a.gate + static_cast<int64_t>(sample) * a.gate_stride : nullptr, kg, 1.0f);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) kg[i] *= k;
+    const uint32_t step = a.chunks * kRows;
+    // every lane of a workgroup-wide row takes part in each round
+    for (uint32_t t = chunk * kRows + threadIdx.x / G; t < a.T; t += step) {
+        const int64_t row = (static_cast<int64_t>(sample) * a.T + t) * a.C;
+        float x[kN], y[kN];
+        lane.load(static_cast<const Tx*>(a.x) + row, x);
+        lane.load(static_cast<const Ty*>(a.y) + row, y);
+        if (a.post) {
+            float pw[kN], pb[kN];
+            lane.load(a.pw, pw, 1.0f);
+            lane.load(a.pb, pb);
+            lane.normalise(y, a.C, a.rms, a.post_eps, lds);
+#pragma unroll
+            for (int i = 0; i < kN; ++i) y[i] = __builtin_fmaf(y[i], pw[i], pb[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kN; ++i) x[i] = __builtin_fmaf(kg[i], y[i], x[i]);
+        lane.store(static_cast<Tx*>(a.sum) + row, x);
+        lane.normalise(x, a.C, a.rms, a.eps, lds);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) x[i] = __builtin_fmaf(x[i], w[i], b[i]);
+        lane.store(static_cast<Ty*>(a.out) + row, x);
+    }
+}
+
+template <typename Tx, typename Ty, int E, int NV, int G>
+__global__ void __launch_bounds__(kThreads) residual_norm_grad_kernel(const NormArgs a) {
+    constexpr int kRows = kThreads / G, kN = NV * E, kCols = G * kN;
+    __shared__ float lds[kRows > 1 ? kThreads * kN : 4];
+    const Lane<E, NV, G> lane(a.C);
+    const uint32_t sample = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+    const float k = a.scale != nullptr ? a.scale[sample] : 1.0f;
+    const float* gate = a.gate != nullptr ? a.gate + static_cast<int64_t>(sample) * a.gate_stride : nullptr;
+    float sums[kSums][kN] = {};
+    const uint32_t step = a.chunks * kRows;
+    for (uint32_t t = chunk * kRows + threadIdx.x / G; t < a.T; t += step) {
+        const int64_t row = (static_cast<int64_t>(sample) * a.T + t) * a.C;
+        float n[kN], y[kN], gx[kN], kg[kN], p[kN], yr = 0.0f;
+        lane.load(static_cast<const Tx*>(a.x) + row, n);
+        lane.load(static_cast<const Ty*>(a.y) + row, y);
+        lane.load(a.gout != nullptr ? static_cast<const Ty*>(a.gout) + row : nullptr, gx);
+        lane.load(gate, kg, 1.0f);
+        if (a.post) yr = lane.normalise(y, a.C, a.rms, a.post_eps, lds);
+        float u[kN];
+        if (a.post) {
+            lane.load(a.pw, p, 1.0f);
+            lane.load(a.pb, u);
+#pragma unroll
+            for (int i = 0; i < kN; ++i) u[i] = __builtin_fmaf(y[i], p[i], u[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) u[i] = y[i];
+        }
+#pragma unroll
+        for (int i = 0; i < kN; ++i) n[i] = __builtin_fmaf(k * kg[i], u[i], n[i]);
+        const float r = lane.normalise(n, a.C, a.rms, a.eps, lds);
+        float w[kN];
+        lane.load(a.w, w, 1.0f);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            sums[0][i] = __builtin_fmaf(gx[i], n[i], sums[0][i]);
+            sums[1][i] += gx[i];
+            gx[i] *= w[i];
+        }
+        lane.normalise_grad(gx, n, r, a.C, a.rms, lds);
+        lane.load(a.gsum != nullptr ? static_cast<const Tx*>(a.gsum) + row : nullptr, n);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) gx[i] += n[i];
+        lane.store(static_cast<Tx*>(a.gx) + row, gx);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            sums[2][i] = __builtin_fmaf(gx[i] * k, u[i], sums[2][i]);
+            gx[i] *= k * kg[i];
+        }
+        if (a.post) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) {
+                sums[3][i] = __builtin_fmaf(gx[i], y[i], sums[3][i]);
+                sums[4][i] += gx[i];
+                gx[i] *= p[i];
+            }
+            lane.normalise_grad(gx, y, yr, a.C, a.rms, lds);
+        }
+        lane.store(static_cast<Ty*>(a.gy) + row, gx);
+    }
+    if (a.partial == nullptr) return;
+    float* to = a.partial + static_cast<int64_t>(blockIdx.x) * kSums * a.C;
+#pragma unroll
+    for (int s = 0; s < kSums; ++s) {
+        // uniform over the launch: the sums that somebody reads
+        if ((s == 2 && a.gate == nullptr) || (s >= 3 && !a.post)) continue;
+        if constexpr (kRows > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    lds[(threadIdx.x / G) * kCols + lane.at[i] + e] = sums[s][i * E + e];
+            }
+            __syncthreads();
+            for (int c = threadIdx.x; c < a.C; c += kThreads) {
+                float v = 0.0f;
+                for (int i = 0; i < kRows; ++i) v += lds[i * kCols + c];
+                to[s * a.C + c] = v;
+            }
+        } else {
+            lane.store(to + s * a.C, sums[s]);
+        }
+    }
+}
+
+// Sums of the partial rows: 16 columns by 16 groups of rows per workgroup.
+struct SumArgs {
+    const float* partial;
+    float* out[kSums];     // null where nobody asked
+    int32_t per_sample[kSums];
+    uint32_t S, chunks;
+    int32_t C;
+};
+
+__global__ void __launch_bounds__(kThreads) residual_norm_sums_kernel(const SumArgs a) {
+    __shared__ float lds[16][17];
+    const int which = static_cast<int>(blockIdx.y);
+    if (a.out[which] == nullptr) return;
+    const uint32_t samples = a.per_sample[which] ? a.S : 1u;
+    if (blockIdx.z >= samples) return;
+    const uint32_t rows = a.per_sample[which] ? a.chunks : a.chunks * a.S;
+    const int c = static_cast<int>(blockIdx.x) * 16 + static_cast<int>(threadIdx.x & 15), part = threadIdx.x >> 4;
+    const float* from = a.partial + (static_cast<int64_t>(blockIdx.z) * rows * kSums + which) * a.C + c;
+    float v = 0.0f;
+    if (c < a.C) {
+#pragma unroll 4
+        for (uint32_t r = part; r < rows; r += 16) v += from[static_cast<int64_t>(r) * kSums * a.C];
+    }
+    lds[part][threadIdx.x & 15] = v;
+    __syncthreads();
+    if (part != 0 || c >= a.C) return;
+    v = 0.0f;
+    for (int i = 0; i < 16; ++i) v += lds[i][threadIdx.x];
+    a.out[which][static_cast<int64_t>(blockIdx.z) * a.C + c] = v;
+}
+
+template <typename Tx, typename Ty, int E, int NV, int G>
+void launch(const NormArgs& a, bool grad, hipStream_t s) {
+    if (grad)
+        residual_norm_grad_kernel<Tx, Ty, E, NV, G><<<a.S * a.chunks, kThreads, 0, s>>>(a);
+    else
+        residual_norm_kernel<Tx, Ty, E, NV, G><<<a.S * a.chunks, kThreads, 0, s>>>(a);
+}
+
+// Lanes of a row: the fewest that hold it in one vector each, then more
+// vectors.  Rows of other lengths go one channel at a time.
+struct Shape {
+    int E, G;
+};
+Shape shape_of(int64_t C) {
+    if (C % 8 == 0) return {8, C <= 64 ? 8 : C <= 128 ? 16 : C <= 256 ? 32 : C <= 1024 ? 64 : 256};
+    return {1, C <= 64 ? 16 : C <= 1024 ? 64 : 256};
+}
+
+template <typename Tx, typename Ty>
+void launch_shape(const NormArgs& a, bool grad, hipStream_t s) {
+    const int C = a.C;
+    if (C % 8 == 0) {
+        if (C <= 64) return launch<Tx, Ty, 8, 1, 8>(a, grad, s);
+        if (C <= 128) return launch<Tx, Ty, 8, 1, 16>(a, grad, s);
+        if (C <= 256) return launch<Tx, Ty, 8, 1, 32>(a, grad, s);
+        if (C <= 512) return launch<Tx, Ty, 8, 1, 64>(a, grad, s);
+        if (C <= 1024) return launch<Tx, Ty, 8, 2, 64>(a, grad, s);
+        if (C <= 2048) return launch<Tx, Ty, 8, 1, 256>(a, grad, s);
+        if (C <= 4096) return launch<Tx, Ty, 8, 2, 256>(a, grad, s);
+        return launch<Tx, Ty, 8, 4, 256>(a, grad, s);
+    }
+    if (C <= 64) return launch<Tx, Ty, 1, 4, 16>(a, grad, s);
+    if (C <= 256) return launch<Tx, Ty, 1, 4, 64>(a, grad, s);
+    if (C <= 1024) return launch<Tx, Ty, 1, 16, 64>(a, grad, s);
+    return launch<Tx, Ty, 1, 16, 256>(a, grad, s);
+}
+
+int dispatch(const NormArgs& a, int32_t x_dtype, int32_t dtype, bool grad, hipStream_t s, const char* what) {
+    if (x_dtype == CRUMPET_DTYPE_F32) {
+        if (dtype == CRUMPET_DTYPE_F32) launch_shape<float, float>(a, grad, s);
+        else if (dtype == CRUMPET_DTYPE_F16) launch_shape<float, _Float16>(a, grad, s);
+        else launch_shape<float, __bf16>(a, grad, s);
+    } else if (dtype == CRUMPET_DTYPE_F16) {
+        launch_shape<_Float16, _Float16>(a, grad, s);
+    } else {
+        launch_shape<__bf16, __bf16>(a, grad, s);
+    }
+    return check_launch(what);
+}
+
+int check(int32_t x_dtype, int32_t dtype, int64_t samples, int64_t tokens, int64_t C, int32_t kind, const char* what) {
+    if (dtype < 0 || dtype > 2 || x_dtype < 0 || x_dtype > 2)
+        return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: unknown dtype code", what);
+    if (x_dtype != dtype && x_dtype != CRUMPET_DTYPE_F32)
+        return fail(CRUMPET_ERR_UNSUPPORTED, "%s: x is float32 or of the branch's type", what);
+    if (kind != 0 && kind != 1) return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: norm is 0 (layer) or 1 (rms)", what);
+    if (samples < 0 || tokens < 0) return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: negative size", what);
+    if (C < 1 || C > 8192 || (C % 8 != 0 && C > 4096))
+        return fail(CRUMPET_ERR_UNSUPPORTED, "%s: C = %lld is outside 1 .. 8192 (4096 where no multiple of 8)", what,
+                    (long long)C);
+    if (samples >= (int64_t(1) << 20) || tokens >= (int64_t(1) << 31))
+        return fail(CRUMPET_ERR_UNSUPPORTED, "%s: more than 2^20 samples or 2^31 tokens", what);
+    return CRUMPET_OK;
+}
+
+bool misaligned(std::initializer_list<const void*> ptrs, int64_t C) {
+    if (C % 8 != 0) return false;  // one channel at a time
+    for (const void* p : ptrs)
+        if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return true;
+    return false;
+}
+
+// Workgroups of a sample: about 2048 in all, none without a row.
+uint32_t chunks_of(int64_t samples, int64_t tokens, int64_t C) {
+    const int64_t rows = kThreads / shape_of(C).G;
+    const int64_t most = (tokens + rows - 1) / rows;
+    return static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(most, (2048 + samples - 1) / samples)));
+}
+
+}  // namespace
+}  // namespace crumpet
+
+using namespace crumpet;
+
+extern "C" int crumpet_residual_norm(void* sum, void* out, const void* x, int32_t x_dtype, const void* y, int32_t dtype,
+                                     int64_t samples, int64_t tokens, int64_t C, int32_t norm, int32_t post,
+                                     const float* post_weight, const float* post_bias, const float* gate,
+                                     int32_t gate_per_sample, const float* scale, const float* weight,
+                                     const float* bias, float eps, void* stream) {
+    const char* what = "residual_norm";
+    const int st = check(x_dtype, dtype, samples, tokens, C, norm, what);
+    if (st != CRUMPET_OK) return st;
+    if (samples == 0 || tokens == 0) return CRUMPET_OK;
+    if (sum == nullptr || out == nullptr || x == nullptr || y == nullptr)
+        return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: null tensor", what);
+    if (misaligned({sum, out, x, y, post_weight, post_bias, gate, weight, bias}, C))
+        return fail(CRUMPET_ERR_UNSUPPORTED, "%s: pointers must be 16-byte aligned where C is a multiple of 8", what);
+    NormArgs a = {};
+    a.x = x, a.y = y, a.pw = post_weight, a.pb = post_bias, a.gate = gate, a.scale = scale, a.w = weight, a.b = bias;
+    a.sum = sum, a.out = out;
+    a.S = static_cast<uint32_t>(samples), a.T = static_cast<uint32_t>(tokens), a.C = static_cast<int32_t>(C);
+    a.chunks = chunks_of(samples, tokens, C);
+    a.gate_stride = gate_per_sample ? a.C : 0;
+    a.post = post, a.rms = norm, a.eps = eps, a.post_eps = eps;
+    return dispatch(a, x_dtype, dtype, false, static_cast<hipStream_t>(stream), what);
+}
+
+extern "C" int64_t crumpet_residual_norm_workspace(int64_t samples, int64_t tokens, int64_t C) {
+    if (samples < 0 || samples >= (int64_t(1) << 20) || tokens < 0 || tokens >= (int64_t(1) << 31) || C < 1 || C > 8192)
+        return -1;
+    if (samples == 0 || tokens == 0) return 0;
+    return samples * chunks_of(samples, tokens, C) * kSums * C * static_cast<int64_t>(sizeof(float));
+}
+
+extern "C" int crumpet_residual_norm_backward(
+    void* grad_x, void* grad_y, float* grad_weight, float* grad_bias, float* grad_gate, float* grad_post_weight,
+    float* grad_post_bias, const void* grad_sum, const void* grad_out, const void* x, int32_t x_dtype, const void* y,
+    int32_t dtype, int64_t samples, int64_t tokens, int64_t C, int32_t norm, int32_t post, const float* post_weight,
+    const float* post_bias, const float* gate, int32_t gate_per_sample, const float* scale, const float* weight,
+    float eps, void* workspace, void* stream) {
+    const char* what = "residual_norm_backward";
+    const int st = check(x_dtype, dtype, samples, tokens, C, norm, what);
+    if (st != CRUMPET_OK) return st;
+    if (samples == 0 || tokens == 0) return CRUMPET_OK;
+    if (grad_x == nullptr || grad_y == nullptr || x == nullptr || y == nullptr)
+        return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: null tensor", what);
+    if (misaligned({grad_x, grad_y, grad_sum, grad_out, x, y, post_weight, post_bias, gate, weight}, C))
+        return fail(CRUMPET_ERR_UNSUPPORTED, "%s: pointers must be 16-byte aligned where C is a multiple of 8", what);
+    if ((grad_gate != nullptr && gate == nullptr) || ((grad_post_weight != nullptr || grad_post_bias != nullptr) && !post))
+        return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: gradient of a parameter that is not there", what);
+    if (gate_per_sample && samples > 65535)
+        return fail(CRUMPET_ERR_UNSUPPORTED, "%s: more than 65535 samples with a gate of their own", what);
+    const bool sums = grad_weight != nullptr || grad_bias != nullptr || grad_gate != nullptr ||
+                      grad_post_weight != nullptr || grad_post_bias != nullptr;
+    if (sums && workspace == nullptr) return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: null workspace", what);
+    NormArgs a = {};
+    a.x = x, a.y = y, a.pw = post_weight, a.pb = post_bias, a.gate = gate, a.scale = scale, a.w = weight;
+    a.gsum = grad_sum, a.gout = grad_out, a.gx = grad_x, a.gy = grad_y;
+    a.partial = sums ? static_cast<float*>(workspace) : nullptr;
+    a.S = static_cast<uint32_t>(samples), a.T = static_cast<uint32_t>(tokens), a.C = static_cast<int32_t>(C);
+    a.chunks = chunks_of(samples, tokens, C);
+    a.gate_stride = gate_per_sample ? a.C : 0;
+    a.post = post, a.rms = norm, a.eps = eps, a.post_eps = eps;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int rc = dispatch(a, x_dtype, dtype, true, s, what);
+    if (rc != CRUMPET_OK || !sums) return rc;
+    SumArgs f = {};
+    f.partial = a.partial;
+    float* outs[kSums] = {grad_weight, grad_bias, grad_gate, grad_post_weight, grad_post_bias};
+    for (int i = 0; i < kSums; ++i) f.out[i] = outs[i];
+    f.per_sample[2] = gate_per_sample;
+    f.S = a.S, f.chunks = a.chunks, f.C = a.C;
+    const uint32_t deep = grad_gate != nullptr && gate_per_sample ? a.S : 1u;
+    residual_norm_sums_kernel<<<dim3((a.C + 15) / 16, kSums, deep), kThreads, 0, s>>>(f);
+    return check_launch(what);
+}

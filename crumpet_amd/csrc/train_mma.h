@@ -1,0 +1,122 @@
+// 16x16 matrix products of the training kernels (gfx950), one wave each.
+//
+// Layout of v_mfma_f32_16x16x16 and of the 16-deep product made of four
+// v_mfma_f32_16x16x4_f32: lane (col = lane & 15, g = lane >> 4) holds
+//   A[m = col][k = 4 g + e],  B[k = 4 g + e][n = col],  e = 0..3,
+//   D[m = 4 g + r][n = col],  r = 0..3.
+// D has the form of a B operand whose depth is D's row, so a product's result
+// feeds the next one without leaving the registers.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "crumpet_common.h"
+#include "crumpet_hip.h"
+
+namespace crumpet {
+namespace train {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+struct Mma;
+
+template <>
+struct Mma<_Float16> {
+    typedef _Float16 x4 __attribute__((ext_vector_type(4)));
+    typedef _Float16 x8 __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f32x4 mma16(x4 a, x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x4 mma32(x8 a, x8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
+
+template <>
+struct Mma<__bf16> {
+    typedef __bf16 x4 __attribute__((ext_vector_type(4)));
+    typedef __bf16 x8 __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f32x4 mma16(x4 a, x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(i16x4, a), __builtin_bit_cast(i16x4, b), c,
+                                                         0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x4 mma32(x8 a, x8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+};
+
+template <>
+struct Mma<float> {
+    typedef f32x4 x4;
+    static __device__ __forceinline__ f32x4 mma16(x4 a, x4 b, f32x4 c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::x4 load4(const T* p) {
+    return *reinterpret_cast<const typename Mma<T>::x4*>(p);
+}
+
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::x4 round4(f32x4 v) {
+    typename Mma<T>::x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = static_cast<T>(v[e]);
+    return o;
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4 wide4(typename Mma<T>::x4 v) {
+    f32x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = static_cast<float>(v[e]);
+    return o;
+}
+
+// The lane's A fragment of the transpose of rows row0 .. row0 + 15 at columns
+// c0 .. c0 + 15 of a row-major LDS tile: [row0 + 4 g + e][c0 + col].  The
+// 16-bit transpose read hands lane (col, g) element col % 4 of the 8-byte
+// vectors that lanes 4 e + col / 4 of its group address.  fp32 reads one value
+// at a time.
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::x4 load_transposed(const T* tile, int ld, int row0, int c0, int col, int g) {
+    if constexpr (sizeof(T) == 2) {
+        typedef __attribute__((address_space(3))) i16x4 LdsI16x4;
+        const T* at = tile + (row0 + 4 * g + (col >> 2)) * ld + c0 + 4 * (col & 3);
+        const i16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsI16x4*)(const_cast<T*>(at)));
+        return __builtin_bit_cast(typename Mma<T>::x4, r);
+    } else {
+        typename Mma<T>::x4 r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = tile[(row0 + 4 * g + e) * ld + c0 + col];
+        return r;
+    }
+}
+
+// Over the 4 lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48).
+__device__ __forceinline__ float sum_groups(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+__device__ __forceinline__ float max_groups(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
+}
+
+__device__ __forceinline__ float load_float(const void* p, int32_t dtype, int64_t i) {
+    if (dtype == CRUMPET_DTYPE_F32) return static_cast<const float*>(p)[i];
+    if (dtype == CRUMPET_DTYPE_F16) return static_cast<float>(static_cast<const _Float16*>(p)[i]);
+    return static_cast<float>(static_cast<const __bf16*>(p)[i]);
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+}  // namespace
+}  // namespace train
+}  // namespace crumpet

@@ -402,6 +402,120 @@ CRUMPET_API int crumpet_rows_linear(void* out, int32_t out_dtype, const void* x,
                                     int64_t rows, int64_t K, const void* weight, const void* bias,
                                     int64_t n_out, int32_t activation, const void* residual, void* stream);
 
+/*
+ * A learned bias by buckets: out[h, p] = table[index[p], h] over `pairs`
+ * query-key pairs; table [buckets, heads], out [heads, pairs], both of
+ * `dtype`.  An index outside the table reads as 0.
+ *
+ * The backward pass takes the pairs sorted by bucket (order [pairs], stable)
+ * and cut into segments of at most crumpet_bucket_segment() sorted pairs, none
+ * across a bucket: segments [segment_count, 2] hold the first and one past the
+ * last.  firsts NULL: one segment for every bucket, in order.  Else firsts
+ * [buckets + 1] says where each bucket's segments begin, and workspace holds
+ * segment_count * heads floats.  fp32 sums in a fixed order, one rounding.
+ *
+ * No counterpart in the reference, whose patch gathers the bias with torch
+ * indexing (torch-ext/crumpet/monai_patch.py:157-162).
+ */
+CRUMPET_API int64_t crumpet_bucket_segment(void);
+CRUMPET_API int crumpet_bucket_bias(void* out, const void* table, int32_t dtype, const int32_t* index,
+                                    int64_t buckets, int64_t heads, int64_t pairs, void* stream);
+CRUMPET_API int crumpet_bucket_bias_backward(void* grad_table, const void* grad, int32_t dtype, int64_t buckets,
+                                             int64_t heads, int64_t pairs, const int32_t* order,
+                                             const int32_t* segments, int64_t segment_count, const int32_t* firsts,
+                                             void* workspace, void* stream);
+
+/*
+ * Window attention for training, over qkv [B, N, 3, heads, head_dim] (window
+ * and token strides in elements, multiples of 16 bytes; the rest dense):
+ *   S = scale q k^T + bias[h] + mask,  out[b, :, h] = softmax(S) v
+ * bias [heads, N, N] fp32.  mask NULL, or [mask_batch, N, N] with rows dense
+ * and mask_stride elements between masks (window b reads mask b mod
+ * mask_batch, which divides B); region NULL, or the shifted-window mask of a
+ * volume: nine numbers D, H, W, ws_d, ws_h, ws_w, ss_d, ss_h, ss_w (window b is
+ * window b mod nW, as in crumpet_fused_swin_attention_shifted).  A row whose
+ * scores are all -inf gives zeros and no gradients.
+ *
+ * For the backward pass the forward pass also writes row_max and row_inv [B,
+ * heads, N] (largest score, 1 / sum of exponentials; both may be NULL
+ * otherwise) and, for 16-bit types, out_rest like out: what out's rounding
+ * left, so that the row sums dO . out, which enter the fp32 gradient of the
+ * bias, are those of the unrounded output.  grad_bias [heads, N, N] fp32 or
+ * NULL.  workspace: crumpet_window_attention_workspace bytes, 16-byte aligned.
+ *
+ * No counterpart in the reference, which is forward-only (README.md:152).
+ */
+CRUMPET_API int crumpet_window_attention(void* out, void* out_rest, float* row_max, float* row_inv, const void* qkv,
+                                         const int64_t qkv_strides[2], int32_t dtype, int64_t B, int64_t heads,
+                                         int64_t N, int64_t head_dim, const float* bias, const void* mask,
+                                         int32_t mask_dtype, int64_t mask_batch, int64_t mask_stride,
+                                         const int64_t* region, float scale, void* stream);
+CRUMPET_API int64_t crumpet_window_attention_workspace(int64_t B, int64_t heads, int64_t N);
+CRUMPET_API int crumpet_window_attention_backward(void* grad_qkv, float* grad_bias, const void* grad_out,
+                                                  const void* out, const void* out_rest, const float* row_max,
+                                                  const float* row_inv, const void* qkv,
+                                                  const int64_t qkv_strides[2], int32_t dtype, int64_t B,
+                                                  int64_t heads, int64_t N, int64_t head_dim, const float* bias,
+                                                  const void* mask, int32_t mask_dtype, int64_t mask_batch,
+                                                  int64_t mask_stride, const int64_t* region, float scale,
+                                                  void* workspace, void* stream);
+
+/*
+ * The residual sum of a block's branch with the norms around it, over
+ * [samples, tokens, C]:
+ *   y' = post ? norm(y) post_weight + post_bias : y
+ *   sum = x + scale[sample] gate y',   out = norm(sum) weight + bias
+ * norm 0: LayerNorm, 1: RMS norm, both with eps.  x and sum are x_dtype
+ * (float32 or `dtype`), y and out `dtype`; parameters fp32, each may be NULL;
+ * gate [C], or [samples, C] with gate_per_sample; scale [samples] or NULL.
+ * out comes from the unrounded sum.  C up to 8192, 4096 where it is no
+ * multiple of 8; pointers 16-byte aligned where it is one.
+ *
+ * The backward pass reads the inputs again (nothing else is kept); grad_sum or
+ * grad_out may be NULL (no gradient from there), and so may each parameter's
+ * gradient.  workspace: crumpet_residual_norm_workspace bytes where any
+ * parameter's gradient is asked for.
+ *
+ * No counterpart in the reference, which leaves both to PyTorch.
+ */
+CRUMPET_API int crumpet_residual_norm(void* sum, void* out, const void* x, int32_t x_dtype, const void* y,
+                                      int32_t dtype, int64_t samples, int64_t tokens, int64_t C, int32_t norm,
+                                      int32_t post, const float* post_weight, const float* post_bias,
+                                      const float* gate, int32_t gate_per_sample, const float* scale,
+                                      const float* weight, const float* bias, float eps, void* stream);
+CRUMPET_API int64_t crumpet_residual_norm_workspace(int64_t samples, int64_t tokens, int64_t C);
+CRUMPET_API int crumpet_residual_norm_backward(
+    void* grad_x, void* grad_y, float* grad_weight, float* grad_bias, float* grad_gate, float* grad_post_weight,
+    float* grad_post_bias, const void* grad_sum, const void* grad_out, const void* x, int32_t x_dtype, const void* y,
+    int32_t dtype, int64_t samples, int64_t tokens, int64_t C, int32_t norm, int32_t post, const float* post_weight,
+    const float* post_bias, const float* gate, int32_t gate_per_sample, const float* scale, const float* weight,
+    float eps, void* workspace, void* stream);
+
+/*
+ * y = act(x) weight^T + bias with act the identity (activation 0) or the exact
+ * GELU (1), x [rows, K], weight [n_out, K], bias [n_out] or NULL, all of
+ * `dtype` (float16 or bfloat16); fp32 accumulation, one rounding.  codes
+ * [rows, K] and exponents [rows, ceil(K / 32)] (both or neither) receive x in 8
+ * bits: codes times 2^e for every 32 columns of a row, e the least integer >=
+ * -126 with 127 2^e >= their largest magnitude; -128 marks a group that is
+ * not finite, kept as NaN.
+ *
+ * The backward pass: grad_x = (grad_y weight) act'(x^), grad_weight = grad_y^T
+ * act(x^), grad_bias = sum of grad_y, each optional, with x^ the 8-bit copy.
+ * K and n_out multiples of 16 up to 65536; pointers 16-byte aligned (the
+ * exponents', grad_weight and grad_bias any).
+ *
+ * No counterpart in the reference.
+ */
+CRUMPET_API int crumpet_linear_8bit(void* y, int8_t* codes, int8_t* exponents, const void* x, int32_t dtype,
+                                    int64_t rows, int64_t K, const void* weight, const void* bias, int64_t n_out,
+                                    int32_t activation, void* stream);
+CRUMPET_API int64_t crumpet_linear_8bit_workspace(int64_t rows, int64_t K, int64_t n_out);
+CRUMPET_API int crumpet_linear_8bit_backward(void* grad_x, void* grad_weight, void* grad_bias, const void* grad_y,
+                                             int32_t dtype, const int8_t* codes, const int8_t* exponents,
+                                             int64_t rows, int64_t K, const void* weight, int64_t n_out,
+                                             int32_t activation, void* workspace, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif
