@@ -38,6 +38,8 @@ HIP_SOURCES = [
     "attention_chunk.hip",
     "window_linear.hip", "block_tail.hip",
     "attention_train.hip", "attention_train_f16.hip", "attention_train_bf16.hip", "attention_train_f32.hip",
+    "attention_train_tuned_f16.hip", "attention_train_tuned_bf16.hip",
+    "attention_train_tuned_f16_mask.hip", "attention_train_tuned_bf16_mask.hip",
     "bias_buckets.hip", "residual_norm.hip", "linear_8bit.hip",
 ]
 BINDING_SOURCES = ["torch_binding.cpp", "training_binding.cpp"]

@@ -34,9 +34,11 @@ struct AttnArgs {
     int32_t mask_dtype, mode;
     uint32_t mask_batch;
     Region region;
+    uint32_t grid[3];           // windows per axis, region mask
     void* out;                  // [B, N, H, D]
     void* out_lo;               // what out's rounding left, 16-bit types only
-    float* row_max;             // [B, H, N]; 0 where a row has no keys
+    float* row_max;             // [B, H, N]; 0 where a row has no keys.  Largest score; the tuned kernels
+                                // without a mask tensor keep it in units of 1 / scale
     float* row_inv;             // [B, H, N] 1 / sum exp(S - max); 0 without keys
     const void* grad_out;       // [B, N, H, D]
     float* delta;               // [B, H, N]
@@ -46,6 +48,46 @@ struct AttnArgs {
     int32_t H, N;
     float scale;
 };
+
+// ---- the bias-stationary kernels (attention_train_tuned.h) -------------------------
+
+// Windows in the order of their kind.  Region classes: which axes the window
+// is last on, of those that are shifted (kind t has start[t + 1] - start[t]
+// windows over all volumes).  Mask tensors: the windows of mask 0, then of
+// mask 1, ...
+struct Order {
+    uint32_t start[9];
+    FastDiv per[8], hw[8], w[8];  // windows of a kind per volume, per plane, per row
+    uint32_t gh, gw, windows;     // grid of a volume
+    uint32_t last[3];
+    FastDiv share;                // windows of one mask
+};
+
+// Workgroups: a group of row tiles of one head, and one of `ranges` ranges of
+// `per` windows.
+struct Walk {
+    uint32_t groups, ranges, per;
+};
+
+enum TunedPass { kForwardPass, kQueryPass, kKeyPass };
+
+// Tiles of 16 tokens that the kernels are compiled for.
+constexpr int tuned_tiles(int N) {
+    return N <= 64 ? 4 : N <= 128 ? 8 : N <= 224 ? 14 : N <= 352 ? 22 : 32;
+}
+// Waves of a workgroup, one tile each.
+constexpr int tuned_waves(int tiles, TunedPass pass) {
+    return tiles == 22 ? (pass == kQueryPass ? 8 : 11) : tiles == 14 ? 7 : tiles == 32 && pass == kQueryPass ? 4
+           : tiles < 8 ? tiles : 8;
+}
+Walk tuned_walk(uint32_t B, int H, int N, TunedPass pass);
+
+int attention_tuned_f16(const AttnArgs& a, const Order& o, int D, bool grad, void* stream);
+int attention_tuned_f16_mask(const AttnArgs& a, const Order& o, int D, bool grad, void* stream);
+int attention_tuned_bf16(const AttnArgs& a, const Order& o, int D, bool grad, void* stream);
+int attention_tuned_bf16_mask(const AttnArgs& a, const Order& o, int D, bool grad, void* stream);
+
+// ---- the general kernels (attention_train_kernels.h) -----------------------------------
 
 // Per element type (attention_train_{f16,bf16,f32}.hip); D one of 16, 32, 64,
 // 128.  They return a status.

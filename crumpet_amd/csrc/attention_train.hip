@@ -34,6 +34,14 @@ uint32_t bias_chunks(int64_t B, int64_t H, int64_t N) {
 
 int64_t rounded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
+// The bias-stationary kernels: 16-bit types, head dims 16 and 32, up to 512
+// tokens.  Without a mask tensor they fold the scale into the bias, which
+// needs a scale whose inverse is an ordinary number.
+bool use_tuned(const AttnArgs& a, int32_t dtype, int64_t D) {
+    const bool folds = a.scale >= 0x1p-20f && a.scale <= 0x1p20f;
+    return dtype != CRUMPET_DTYPE_F32 && (D == 16 || D == 32) && a.N <= 512 && (folds || a.mode == kTensorMask);
+}
+
 int check(AttnArgs& a, int32_t dtype, int64_t B, int64_t H, int64_t N, int64_t D, const int64_t strides[2],
           const float* bias, const void* mask, int32_t mask_dtype, int64_t mask_batch, int64_t mask_stride,
           const int64_t* region, float scale, const char* what) {
@@ -90,9 +98,47 @@ int check(AttnArgs& a, int32_t dtype, int64_t B, int64_t H, int64_t N, int64_t D
             r.from[i] = static_cast<int32_t>(ws[i] - ss[i]);
             r.last[i] = ss[i] > 0 ? static_cast<int32_t>(nw[i] - 1) : -1;
         }
-        if (ss[0] > 0 || ss[1] > 0 || ss[2] > 0) a.mode = kRegionMask;
+        if (ss[0] > 0 || ss[1] > 0 || ss[2] > 0) {
+            a.mode = kRegionMask;
+            for (int i = 0; i < 3; ++i) a.grid[i] = static_cast<uint32_t>(nw[i]);
+        }
     }
+    if (use_tuned(a, dtype, D)) a.chunks = tuned_walk(a.B, a.H, a.N, kQueryPass).ranges;
     return CRUMPET_OK;
+}
+
+Order order_of(const AttnArgs& a) {
+    Order o;
+    o.share.init(a.mode == kTensorMask ? a.B / a.mask_batch : 1);
+    // without a mask: one kind, one row of windows
+    uint32_t n[3] = {1, 1, a.B};
+    bool shifted[3] = {};
+    if (a.mode == kRegionMask) {
+        for (int i = 0; i < 3; ++i) n[i] = a.grid[i], shifted[i] = a.region.last[i] >= 0;
+    }
+    o.gh = n[1], o.gw = n[2], o.windows = n[0] * n[1] * n[2];
+    const uint32_t volumes = a.B / o.windows;
+    o.start[0] = 0;
+    for (uint32_t t = 0; t < 8; ++t) {
+        uint32_t m[3];
+        for (int i = 0; i < 3; ++i) m[i] = t >> i & 1 ? (shifted[i] ? 1 : 0) : shifted[i] ? n[i] - 1 : n[i];
+        const uint32_t count = m[0] * m[1] * m[2];
+        o.start[t + 1] = o.start[t] + count * volumes;
+        o.per[t].init(std::max(1u, count));
+        o.hw[t].init(std::max(1u, m[1] * m[2]));
+        o.w[t].init(std::max(1u, m[2]));
+    }
+    for (int i = 0; i < 3; ++i) o.last[i] = n[i] - 1;
+    return o;
+}
+
+int run_tuned(const AttnArgs& a, int32_t dtype, int D, bool grad, void* stream) {
+    const Order o = order_of(a);
+    if (a.mode == kTensorMask)
+        return dtype == CRUMPET_DTYPE_F16 ? attention_tuned_f16_mask(a, o, D, grad, stream)
+                                          : attention_tuned_bf16_mask(a, o, D, grad, stream);
+    return dtype == CRUMPET_DTYPE_F16 ? attention_tuned_f16(a, o, D, grad, stream)
+                                      : attention_tuned_bf16(a, o, D, grad, stream);
 }
 
 bool misaligned(std::initializer_list<const void*> ptrs) {
@@ -102,6 +148,19 @@ bool misaligned(std::initializer_list<const void*> ptrs) {
 }
 
 }  // namespace
+
+// As many ranges as keep every CU's workgroups in one round.
+Walk tuned_walk(uint32_t B, int H, int N, TunedPass pass) {
+    const int waves = tuned_waves(tuned_tiles(N), pass), tiles = (N + 15) / 16;
+    Walk w;
+    w.groups = static_cast<uint32_t>((tiles + waves - 1) / waves);
+    const uint32_t units = w.groups * static_cast<uint32_t>(H), resident = tuned_tiles(N) <= 8 ? 4 : tuned_tiles(N) == 14 ? 2 : 1;
+    const uint32_t ranges = std::max(1u, std::min(B, 256 * resident / units));
+    w.per = (B + ranges - 1) / ranges;
+    w.ranges = (B + w.per - 1) / w.per;
+    return w;
+}
+
 }  // namespace train
 }  // namespace crumpet
 
@@ -124,6 +183,7 @@ extern "C" int crumpet_window_attention(void* out, void* out_rest, float* row_ma
         return fail(CRUMPET_ERR_UNSUPPORTED, "%s: pointers must be 16-byte aligned", what);
     a.out = out, a.out_lo = out_rest, a.row_max = row_max, a.row_inv = row_inv, a.qkv = qkv;
     const int D = static_cast<int>(head_dim);
+    if (use_tuned(a, dtype, D)) return run_tuned(a, dtype, D, false, stream);
     if (dtype == CRUMPET_DTYPE_F16) return attention_forward_f16(a, D, stream);
     if (dtype == CRUMPET_DTYPE_BF16) return attention_forward_bf16(a, D, stream);
     return attention_forward_f32(a, D, stream);
@@ -132,7 +192,11 @@ extern "C" int crumpet_window_attention(void* out, void* out_rest, float* row_ma
 extern "C" int64_t crumpet_window_attention_workspace(int64_t B, int64_t heads, int64_t N) {
     if (B < 0 || heads < 0 || N < 0 || B >= (int64_t(1) << 31) || heads > 4096 || N > 16384) return -1;
     if (B == 0 || heads == 0 || N == 0) return 0;
-    return rounded(B * heads * N * 4) + bias_chunks(B, heads, N) * heads * N * N * 4;
+    uint32_t chunks = bias_chunks(B, heads, N);
+    if (N <= 512)
+        chunks = std::max(chunks, tuned_walk(static_cast<uint32_t>(B), static_cast<int>(heads), static_cast<int>(N),
+                                             kQueryPass).ranges);
+    return rounded(B * heads * N * 4) + chunks * heads * N * N * 4;
 }
 
 extern "C" int crumpet_window_attention_backward(void* grad_qkv, float* grad_bias, const void* grad_out, const void* out,
@@ -161,7 +225,8 @@ extern "C" int crumpet_window_attention_backward(void* grad_qkv, float* grad_bia
     if (grad_bias != nullptr) a.grad_bias = a.chunks == 1 ? grad_bias : partial;
     const int D = static_cast<int>(head_dim);
     int rc;
-    if (dtype == CRUMPET_DTYPE_F16) rc = attention_backward_f16(a, D, stream);
+    if (use_tuned(a, dtype, D)) rc = run_tuned(a, dtype, D, true, stream);
+    else if (dtype == CRUMPET_DTYPE_F16) rc = attention_backward_f16(a, D, stream);
     else if (dtype == CRUMPET_DTYPE_BF16) rc = attention_backward_bf16(a, D, stream);
     else rc = attention_backward_f32(a, D, stream);
     if (rc != CRUMPET_OK || grad_bias == nullptr || a.chunks == 1) return rc;

@@ -437,8 +437,8 @@ CRUMPET_API int crumpet_bucket_bias_backward(void* grad_table, const void* grad,
  * scores are all -inf gives zeros and no gradients.
  *
  * For the backward pass the forward pass also writes row_max and row_inv [B,
- * heads, N] (largest score, 1 / sum of exponentials; both may be NULL
- * otherwise) and, for 16-bit types, out_rest like out: what out's rounding
+ * heads, N] (the softmax statistics, for a backward pass with the same
+ * arguments; both may be NULL otherwise) and, for 16-bit types, out_rest like out: what out's rounding
  * left, so that the row sums dO . out, which enter the fp32 gradient of the
  * bias, are those of the unrounded output.  grad_bias [heads, N, N] fp32 or
  * NULL.  workspace: crumpet_window_attention_workspace bytes, 16-byte aligned.
