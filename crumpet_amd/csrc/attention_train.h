@@ -75,12 +75,27 @@ enum TunedPass { kForwardPass, kQueryPass, kKeyPass };
 constexpr int tuned_tiles(int N) {
     return N <= 64 ? 4 : N <= 128 ? 8 : N <= 224 ? 14 : N <= 352 ? 22 : 32;
 }
-// Waves of a workgroup, one tile each.
-constexpr int tuned_waves(int tiles, TunedPass pass) {
-    return tiles == 22 ? (pass == kQueryPass ? 8 : 11) : tiles == 14 ? 7 : tiles == 32 && pass == kQueryPass ? 4
-           : tiles < 8 ? tiles : 8;
+// Strips of a workgroup, waves that share one (each with its part of the other
+// axis' tiles), waves per SIMD that the registers are allotted for.  A spilled
+// tile costs more than a wave: the query pass keeps 8 registers a tile, the
+// others 4, and about 100 more.  Few strips to a workgroup, so that two or more
+// of them fill a CU and one computes while another waits at its barrier, except
+// at head dim 32, whose rows fill the LDS.  Stage 0 (22 tiles, 1372 windows, 3
+// heads of 16, fp16): query pass 305 us with {2, 2, 2}, 331 with {4, 2, 2}, 435
+// with {4, 1, 1}; key pass 240 with {4, 1, 2}, 264 with {6, 2, 3}; forward 236
+// with {4, 1, 2}, 242 with {6, 2, 3}.
+struct Form {
+    int strips, split, per_simd;
+};
+constexpr Form tuned_form(int tiles, int D, TunedPass pass) {
+    if (tiles <= 8) return {4, 1, 2};
+    if (tiles == 14)
+        return pass == kForwardPass ? Form{4, 2, 2} : pass == kKeyPass ? Form{7, 1, 2} : D == 16 ? Form{3, 2, 2} : Form{4, 2, 2};
+    if (tiles == 22)
+        return pass == kQueryPass ? (D == 16 ? Form{2, 2, 2} : Form{4, 2, 2}) : D == 16 ? Form{4, 1, 2} : Form{8, 1, 2};
+    return pass == kQueryPass ? Form{2, 4, 2} : D == 32 && pass == kKeyPass ? Form{8, 1, 2} : Form{4, 2, 2};
 }
-Walk tuned_walk(uint32_t B, int H, int N, TunedPass pass);
+Walk tuned_walk(uint32_t B, int H, int N, int D, TunedPass pass);
 
 int attention_tuned_f16(const AttnArgs& a, const Order& o, int D, bool grad, void* stream);
 int attention_tuned_f16_mask(const AttnArgs& a, const Order& o, int D, bool grad, void* stream);

@@ -36,8 +36,10 @@ int64_t rounded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // The bias-stationary kernels: 16-bit types, head dims 16 and 32, up to 512
 // tokens.  Without a mask tensor they fold the scale into the bias, which
-// needs a scale whose inverse is an ordinary number.
+// needs a scale whose inverse is an ordinary number.  Offsets in a window's rows
+// take 32 bits there.
 bool use_tuned(const AttnArgs& a, int32_t dtype, int64_t D) {
+    if (a.st < 0 || a.st >= int64_t(1) << 21 || a.H > 4096) return false;
     const bool folds = a.scale >= 0x1p-20f && a.scale <= 0x1p20f;
     return dtype != CRUMPET_DTYPE_F32 && (D == 16 || D == 32) && a.N <= 512 && (folds || a.mode == kTensorMask);
 }
@@ -103,7 +105,7 @@ int check(AttnArgs& a, int32_t dtype, int64_t B, int64_t H, int64_t N, int64_t D
             for (int i = 0; i < 3; ++i) a.grid[i] = static_cast<uint32_t>(nw[i]);
         }
     }
-    if (use_tuned(a, dtype, D)) a.chunks = tuned_walk(a.B, a.H, a.N, kQueryPass).ranges;
+    if (use_tuned(a, dtype, D)) a.chunks = tuned_walk(a.B, a.H, a.N, static_cast<int>(D), kQueryPass).ranges;
     return CRUMPET_OK;
 }
 
@@ -150,11 +152,16 @@ bool misaligned(std::initializer_list<const void*> ptrs) {
 }  // namespace
 
 // As many ranges as keep every CU's workgroups in one round.
-Walk tuned_walk(uint32_t B, int H, int N, TunedPass pass) {
-    const int waves = tuned_waves(tuned_tiles(N), pass), tiles = (N + 15) / 16;
+Walk tuned_walk(uint32_t B, int H, int N, int D, TunedPass pass) {
+    const Form f = tuned_form(tuned_tiles(N), D, pass);
+    const uint32_t tiles = static_cast<uint32_t>((N + 15) / 16);
     Walk w;
-    w.groups = static_cast<uint32_t>((tiles + waves - 1) / waves);
-    const uint32_t units = w.groups * static_cast<uint32_t>(H), resident = tuned_tiles(N) <= 8 ? 4 : tuned_tiles(N) == 14 ? 2 : 1;
+    w.groups = (tiles + f.strips - 1) / f.strips;
+    const uint32_t units = w.groups * static_cast<uint32_t>(H);
+    // workgroups that a CU holds: by waves and by LDS (rows, the strips' sums, the key pass' statistics)
+    const int rows = tuned_tiles(N) * 16, values = D / 4 * (pass == kKeyPass ? 2 : 1) + 2;
+    const int lds = 8 * rows * D + 512 * f.strips * (f.split - 1) * values + (pass == kKeyPass ? 32 * rows : rows);
+    const uint32_t resident = std::max(1, std::min(4 * f.per_simd / (f.strips * f.split), 163840 / lds));
     const uint32_t ranges = std::max(1u, std::min(B, 256 * resident / units));
     w.per = (B + ranges - 1) / ranges;
     w.ranges = (B + w.per - 1) / w.per;
@@ -193,8 +200,8 @@ extern "C" int64_t crumpet_window_attention_workspace(int64_t B, int64_t heads, 
     if (B < 0 || heads < 0 || N < 0 || B >= (int64_t(1) << 31) || heads > 4096 || N > 16384) return -1;
     if (B == 0 || heads == 0 || N == 0) return 0;
     uint32_t chunks = bias_chunks(B, heads, N);
-    if (N <= 512)
-        chunks = std::max(chunks, tuned_walk(static_cast<uint32_t>(B), static_cast<int>(heads), static_cast<int>(N),
+    for (int D = 16; D <= 32 && N <= 512; D *= 2)
+        chunks = std::max(chunks, tuned_walk(static_cast<uint32_t>(B), static_cast<int>(heads), static_cast<int>(N), D,
                                              kQueryPass).ranges);
     return rounded(B * heads * N * 4) + chunks * heads * N * N * 4;
 }

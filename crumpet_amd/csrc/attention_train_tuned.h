@@ -53,19 +53,48 @@ __device__ __forceinline__ Place place_of(const AttnArgs& a, const Order& o, uin
         if (t & 4) ww = o.last[2];
         p.b = outer * o.windows + (wd * o.gh + wh) * o.gw + ww, p.kind = t;
     }
-    p.b = __builtin_amdgcn_readfirstlane(p.b);
-    p.kind = __builtin_amdgcn_readfirstlane(p.kind);
     return p;
 }
+
+// The places of a walk's windows: each lane works out one of the next 64, the
+// divisions of which would hold up every window otherwise.
+template <bool kMask>
+struct Places {
+    Place mine;
+    uint32_t begin, end;
+    __device__ __forceinline__ Places(uint32_t b, uint32_t e) : mine(), begin(b), end(e) {}
+    __device__ __forceinline__ Place at(const AttnArgs& a, const Order& o, uint32_t i) {
+        const uint32_t n = i - begin;
+        if (n % 64 == 0) {
+            const uint32_t w = i + (threadIdx.x & 63);
+            mine = place_of<kMask>(a, o, w < end ? w : end - 1);
+        }
+        Place p;
+        p.b = __builtin_amdgcn_readlane(mine.b, n % 64);
+        p.kind = __builtin_amdgcn_readlane(mine.kind, n % 64);
+        return p;
+    }
+};
 
 template <typename T, int D>
 struct Lds {
     // 16-byte pieces of a row; at head dim 32 they are permuted by the row so
     // that fragment and transpose reads of 16 rows meet distinct banks
-    static __device__ __forceinline__ int at(int row, int c) {
-        if constexpr (D == 16) return row * 16 + c * 8;
-        const int sw = ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
-        return row * 32 + ((c ^ sw) << 3);
+    static __device__ __forceinline__ int piece(int row, int c) {
+        return D == 16 ? c : c ^ (((row >> 2) & 1) << 1 | ((row >> 3) & 1));
+    }
+    static __device__ __forceinline__ int at(int row, int c) { return row * D + piece(row, c) * 8; }
+};
+
+// Two views of a tile for the even and the odd 16 rows: a merged read of both
+// (ds_read2st64_b64) meets the same banks twice and takes 32 cycles for 8.
+template <typename T>
+struct Halves {
+    const T* of[2];
+    __device__ __forceinline__ Halves(const T* tile, int step) {
+        uint32_t other = step;
+        asm volatile("" : "+v"(other));
+        of[0] = tile, of[1] = tile + other;
     }
 };
 
@@ -75,7 +104,7 @@ struct Operand;
 template <typename T>
 struct Operand<T, 16> {
     typename Mma<T>::x4 v;
-    __device__ __forceinline__ void load(const T* row, int g) { v = load4<T>(row + 4 * g); }
+    __device__ __forceinline__ void load(const T* first, uint32_t row, int g) { v = load4<T>(first + (row + 4 * g)); }
     __device__ __forceinline__ void load_lds(const T* tile, int row0, int col, int g) {
         v = load4<T>(tile + (row0 + col) * 16 + 4 * g);
     }
@@ -84,8 +113,8 @@ struct Operand<T, 16> {
 template <typename T>
 struct Operand<T, 32> {
     typename Mma<T>::x8 v;
-    __device__ __forceinline__ void load(const T* row, int g) {
-        v = *reinterpret_cast<const typename Mma<T>::x8*>(row + 8 * g);
+    __device__ __forceinline__ void load(const T* first, uint32_t row, int g) {
+        v = *reinterpret_cast<const typename Mma<T>::x8*>(first + (row + 8 * g));
     }
     __device__ __forceinline__ void load_lds(const T* tile, int row0, int col, int g) {
         v = *reinterpret_cast<const typename Mma<T>::x8*>(tile + Lds<T, 32>::at(row0 + col, g));
@@ -120,33 +149,52 @@ __device__ __forceinline__ typename Mma<T>::x8 transposed_pair(const T* tile, in
     return join<T>(__builtin_bit_cast(typename Mma<T>::x4, r[0]), __builtin_bit_cast(typename Mma<T>::x4, r[1]));
 }
 
-// Rows of one matrix of a window on their way into LDS: each thread's pieces.
+template <typename T, int D>
+__device__ __forceinline__ typename Mma<T>::x4 transposed_one(const T* tile, int row0, int s, int col, int g) {
+    typedef __attribute__((address_space(3))) i16x4 LdsI16x4;
+    const T* at = tile + Lds<T, D>::at(row0 + 4 * g + (col >> 2), 2 * s + ((col & 3) >> 1)) + 4 * (col & 1);
+    return __builtin_bit_cast(typename Mma<T>::x4,
+                              __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsI16x4*)(const_cast<T*>(at))));
+}
+
+// Addresses: a base that is the same for the wave (scalar registers) plus a
+// 32-bit offset of the lane, which stays the same from window to window.
+
+// Rows of one matrix of a window on their way into LDS, without passing through
+// registers: load j of a wave fills the 64 16-byte slots from 64 j, in slot
+// order, with the pieces that belong there.
 template <typename T, int D, int NT, int W>
-struct Pieces {
-    static constexpr int kAll = NT * 16 * (D / 8), kThreads = W * 64, kEach = (kAll + kThreads - 1) / kThreads;
-    typedef typename Mma<T>::x8 X8;
-    X8 v[kEach];
-    __device__ __forceinline__ void load(const T* first, int64_t stride, int N) {
+struct Rows {
+    static constexpr int kLoads = NT * 16 * (D / 8) / 64, kEach = (kLoads + W - 1) / W;
+    uint32_t of[kEach];  // where the lane's pieces lie in the matrix, bytes
+    uint32_t bytes;
+    int wave;
+    __device__ __forceinline__ Rows(uint32_t stride, int N) {
+        wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+        bytes = (static_cast<uint32_t>(N - 1) * stride + D) * sizeof(T);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const int p = threadIdx.x + i * kThreads, r = p / (D / 8), c = p % (D / 8);
-            if (kAll % kThreads != 0 && p >= kAll) break;
-            v[i] = *reinterpret_cast<const X8*>(first + (r < N ? r : N - 1) * stride + c * 8);
+            const int slot = (wave + i * W) * 64 + (threadIdx.x & 63), r = slot / (D / 8);
+            of[i] = (static_cast<uint32_t>(r < N ? r : N - 1) * stride + Lds<T, D>::piece(r, slot % (D / 8)) * 8) * sizeof(T);
         }
     }
-    __device__ __forceinline__ void store(T* lds) const {
+    __device__ __forceinline__ void load(const T* first, uint32_t to) const {
+        const u32x4 buffer = buffer_of(first, bytes);
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int p = threadIdx.x + i * kThreads, r = p / (D / 8), c = p % (D / 8);
-            if (kAll % kThreads != 0 && p >= kAll) break;
-            *reinterpret_cast<X8*>(lds + Lds<T, D>::at(r, c)) = v[i];
-        }
+        for (int i = 0; i < kEach; ++i)
+            if (wave + i * W < kLoads) load_to_lds(buffer, to + (wave + i * W) * 1024, of[i]);
     }
 };
 
 template <typename T>
 __device__ __forceinline__ const T* rows_of(const AttnArgs& a, uint32_t b, int which, int h, int D) {
     return static_cast<const T*>(a.qkv) + static_cast<int64_t>(b) * a.sb + (static_cast<int64_t>(which) * a.H + h) * D;
+}
+
+// First element of a window's and head's rows in [B, N, H, D].
+template <int D>
+__device__ __forceinline__ int64_t heads_row(const AttnArgs& a, uint32_t b, int h) {
+    return (static_cast<int64_t>(b) * a.N * a.H + h) * D;
 }
 
 // Which seams a token lies past, for every token.
@@ -160,11 +208,37 @@ __device__ __forceinline__ void token_sides(const AttnArgs& a, uint8_t* side, in
     }
 }
 
+// v = hi + lo to twice the type's precision: hi rounded towards zero in fp16
+// (one packed conversion; the rest is exact all the same).
+template <typename T>
+__device__ __forceinline__ void split(f32x4 v, typename Mma<T>::x4& hi, typename Mma<T>::x4& lo) {
+    if constexpr (std::is_same<T, _Float16>::value) {
+        typedef __fp16 h16x2 __attribute__((ext_vector_type(2)));
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        const f16x2 a = __builtin_bit_cast(f16x2, static_cast<h16x2>(__builtin_amdgcn_cvt_pkrtz(v[0], v[1])));
+        const f16x2 b = __builtin_bit_cast(f16x2, static_cast<h16x2>(__builtin_amdgcn_cvt_pkrtz(v[2], v[3])));
+        hi = __builtin_shufflevector(a, b, 0, 1, 2, 3);
+        f32x4 rest;
+        // v - hi in one step: v_fma_mix_f32 takes the fp16 half as it is
+        const uint32_t pair[2] = {__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+            asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(rest[e]) : "v"(pair[e >> 1]), "v"(v[e]));
+            asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+                : "=v"(rest[e + 1])
+                : "v"(pair[e >> 1]), "v"(v[e + 1]));
+        }
+        lo = round4<T>(rest);
+    } else {
+        hi = round4<T>(v);
+        lo = round4<T>(v - wide4<T>(hi));
+    }
+}
+
 // The unrolled loops over the tiles are straight-line code, which the compiler
 // would otherwise start all of at once, in registers that it does not have.
 __device__ __forceinline__ void tiles_in_order() {
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
 }
 
 // Computed here, not where it is next used: otherwise the sums of a whole
@@ -175,13 +249,13 @@ __device__ __forceinline__ void settled(V& v) {
 }
 
 template <int NT, bool kKeysInLanes, typename M>
-__device__ __forceinline__ void add_mask(f32x4* tile, const M* mask, int N, int mine, int g) {
-    asm volatile("" : "+v"(mine), "+v"(g));
+__device__ __forceinline__ void add_mask(f32x4* tile, const M* mask, int N, int mine, int first) {
+    asm volatile("" : "+v"(mine), "+v"(first));
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int other = 16 * t + 4 * g + r, o = other < N ? other : N - 1;
+            const int other = 16 * t + first + r, o = other < N ? other : N - 1;
             tile[t][r] += static_cast<float>(mask[kKeysInLanes ? o * N + mine : mine * N + o]);
         }
         tiles_in_order();
@@ -192,19 +266,19 @@ __device__ __forceinline__ void add_mask(f32x4* tile, const M* mask, int N, int 
 // the start of the score product; with a mask tensor: bias + mask, added in
 // score units, so that the type's lowest value stays what it is.  Keys past N
 // are -inf.  kKeysInLanes: a lane's column is its key and its rows are queries.
+// first: the other axis' index of the lane's first value.
 template <int NT, bool kMask, bool kKeysInLanes>
-__device__ __forceinline__ void build_tiles(f32x4* tile, const AttnArgs& a, int h, uint32_t kind, int row, int g,
+__device__ __forceinline__ void build_tiles(f32x4* tile, const AttnArgs& a, int h, uint32_t kind, int mine, int first,
                                             const uint8_t* side, float per_scale) {
     const float* bias = a.bias + static_cast<int64_t>(h) * a.N * a.N;
-    int mine = row < a.N ? row : a.N - 1;
     // keeps the addresses of all tiles from being computed ahead of the walk
     // and held in registers through it
-    asm volatile("" : "+v"(mine), "+v"(g));
+    asm volatile("" : "+v"(mine), "+v"(first));
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int other = 16 * t + 4 * g + r;
+            const int other = 16 * t + first + r;
             const bool in = other < a.N;
             const int o = in ? other : a.N - 1;
             float v = bias[kKeysInLanes ? o * a.N + mine : mine * a.N + o];
@@ -217,14 +291,27 @@ __device__ __forceinline__ void build_tiles(f32x4* tile, const AttnArgs& a, int 
         tiles_in_order();
     }
     if constexpr (kMask) {
-        const int64_t first = static_cast<int64_t>(kind) * a.mask_sb;
+        const int64_t at = static_cast<int64_t>(kind) * a.mask_sb;
         if (a.mask_dtype == CRUMPET_DTYPE_F32)
-            add_mask<NT, kKeysInLanes>(tile, static_cast<const float*>(a.mask) + first, a.N, mine, g);
+            add_mask<NT, kKeysInLanes>(tile, static_cast<const float*>(a.mask) + at, a.N, mine, first);
         else if (a.mask_dtype == CRUMPET_DTYPE_F16)
-            add_mask<NT, kKeysInLanes>(tile, static_cast<const _Float16*>(a.mask) + first, a.N, mine, g);
+            add_mask<NT, kKeysInLanes>(tile, static_cast<const _Float16*>(a.mask) + at, a.N, mine, first);
         else
-            add_mask<NT, kKeysInLanes>(tile, static_cast<const __bf16*>(a.mask) + first, a.N, mine, g);
+            add_mask<NT, kKeysInLanes>(tile, static_cast<const __bf16*>(a.mask) + at, a.N, mine, first);
     }
+}
+
+// Lane (col, g)'s value for row 4 g + r, from the lane of its group that holds it.
+__device__ __forceinline__ float of_row(float v, int r) {
+    const int bits = __float_as_int(v);
+    int got = bits;
+    switch (r) {  // DPP row_newbcast
+        case 0: got = __builtin_amdgcn_update_dpp(0, bits, 0x150, 0xf, 0xf, true); break;
+        case 1: got = __builtin_amdgcn_update_dpp(0, bits, 0x151, 0xf, 0xf, true); break;
+        case 2: got = __builtin_amdgcn_update_dpp(0, bits, 0x152, 0xf, 0xf, true); break;
+        default: got = __builtin_amdgcn_update_dpp(0, bits, 0x153, 0xf, 0xf, true); break;
+    }
+    return __int_as_float(got);
 }
 
 // Beyond this a score's products no longer cancel to a few bits when they are
@@ -259,96 +346,225 @@ struct Exponent {
     }
 };
 
-template <typename T, int D, int NT, int W, bool kMask>
-__global__ void __launch_bounds__(W * 64) attn_forward_tuned_kernel(const AttnArgs a, const Order o, const Walk w) {
+// Where a wave stands: kSplit waves share the 16 rows of a strip, each with
+// kSpan of the NT tiles of the other axis.
+template <int NT, int S, int kSplit>
+struct Share {
+    static constexpr int kSpan = NT / kSplit;
+    int lane, col, g, local, part, row0, row, first;
+    bool active, leads;
+    __device__ __forceinline__ Share(const AttnArgs& a, uint32_t group) {
+        const int wave = threadIdx.x >> 6;
+        lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+        local = wave / kSplit, part = wave % kSplit;
+        const int strip = static_cast<int>(group) * S + local;
+        row0 = strip * 16 + col, row = row0 < a.N ? row0 : a.N - 1;
+        active = strip * 16 < a.N;
+        leads = part == 0;
+        first = part * kSpan;  // first tile of the other axis
+    }
+};
+
+// Sums that the other waves of a strip hand to the one that leads it: written
+// at the end of a window, read after the barrier that ends it, in two copies
+// so that the next window's do not meet them.
+template <int S, int kSplit, int kValues>
+struct Handover {
+    static constexpr int kFloats = kSplit > 1 ? 2 * S * (kSplit - 1) * kValues * 64 : 1;
+    float* lds;
+    int at;
+    __device__ __forceinline__ Handover(float* l, int local, int lane) : lds(l), at(local * (kSplit - 1) * kValues * 64 + lane) {}
+    __device__ __forceinline__ float& value(int copy, int part, int v) const {
+        return lds[copy * S * (kSplit - 1) * kValues * 64 + at + ((part - 1) * kValues + v) * 64];
+    }
+};
+
+// The transposed rows of `count` tiles (1 or 2) at row0, to be added up with
+// weights: acc[d][lane's column] += rows times w.
+template <typename T, int D>
+struct Turned {
+    typename Mma<T>::x8 v[D / 16];
+    __device__ __forceinline__ void load(const T* lds, int row0, int count, int col, int g) {
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+            if (count == 2) {
+                v[d] = transposed_pair<T, D>(lds, row0, d, col, g);
+            } else {
+                const typename Mma<T>::x4 one = transposed_one<T, D>(lds, row0, d, col, g);
+                v[d] = join<T>(one, one);
+            }
+        }
+    }
+    __device__ __forceinline__ void add(f32x4* acc, int count, const typename Mma<T>::x4* w) const {
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+            if (count == 2)
+                acc[d] = Mma<T>::mma32(v[d], join<T>(w[0], w[1]), acc[d]);
+            else
+                acc[d] = Mma<T>::mma16(__builtin_shufflevector(v[d], v[d], 0, 1, 2, 3), w[0], acc[d]);
+        }
+    }
+};
+
+template <typename T, int D, int NT, int S, int kSplit, int kWaves, bool kMask>
+__global__ void __launch_bounds__(S* kSplit * 64) __attribute__((amdgpu_waves_per_eu(kWaves)))
+attn_forward_tuned_kernel(const AttnArgs a, const Order o, const Walk w) {
     typedef typename Mma<T>::x4 X4;
-    constexpr int kTile = NT * 16 * D;
-    constexpr int kOut = D / 16;
+    typedef Share<NT, S, kSplit> Mine;
+    constexpr int kTile = NT * 16 * D, W = S * kSplit, kOut = D / 16, kSpan = Mine::kSpan;
+    typedef Handover<S, kSplit, 4 * kOut + 2> Hand;
     __shared__ __attribute__((aligned(16))) T k_lds[2][kTile];
     __shared__ __attribute__((aligned(16))) T v_lds[2][kTile];
+    __shared__ float hand_lds[Hand::kFloats];
     __shared__ uint8_t side[kMask ? 4 : NT * 16];
     uint32_t range, group;
     int h;
     if (!walk_of(a, w, range, group, h)) return;
     const uint32_t begin = range * w.per, end = std::min(a.B, begin + w.per);
-    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-    const int strip = static_cast<int>(group) * W + (threadIdx.x >> 6);
-    const int q0 = strip * 16 + col, q = q0 < a.N ? q0 : a.N - 1;
-    const bool active = strip * 16 < a.N;
+    const Mine me(a, group);
+    const int col = me.col, g = me.g, q = me.row;
+    const Hand hand(hand_lds, me.local, me.lane);
     const float per_scale = 1.0f / a.scale, c2 = a.scale * kLog2e;
+    const float unit = kMask ? kLog2e : c2;  // of `top`, to log2
     if constexpr (!kMask) token_sides(a, side, std::min(a.N, NT * 16));
-    f32x4 tile[NT];
+    X4 ones;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ones[e] = static_cast<T>(1.0f);
+    f32x4 tile[kSpan];
     uint32_t kind = ~0u;
-    Pieces<T, D, NT, W> kp, vp;
     Operand<T, D> qn;
-    Place p = place_of<kMask>(a, o, begin);
-    kp.load(rows_of<T>(a, p.b, 1, h, D), a.st, a.N);
-    vp.load(rows_of<T>(a, p.b, 2, h, D), a.st, a.N);
-    qn.load(rows_of<T>(a, p.b, 0, h, D) + q * a.st, g);
-    kp.store(k_lds[0]);
-    vp.store(v_lds[0]);
+    Places<kMask> places(begin, end);
+    Place p = places.at(a, o, begin);
+    const Rows<T, D, NT, W> rows(static_cast<uint32_t>(a.st), a.N);
+    const uint32_t mine = static_cast<uint32_t>(q) * static_cast<uint32_t>(a.st);
+    const auto fetch = [&](uint32_t b, int buf) {
+        rows.load(rows_of<T>(a, b, 1, h, D), lds_address(k_lds[0]) + buf * kTile * sizeof(T));
+        rows.load(rows_of<T>(a, b, 2, h, D), lds_address(v_lds[0]) + buf * kTile * sizeof(T));
+        qn.load(rows_of<T>(a, b, 0, h, D), mine, g);
+    };
+    fetch(p.b, 0);
+    f32x4 acc[kOut];
+    float top, total;
+    // joins the strip's parts and stores the window's rows
+    const auto finish = [&](uint32_t b, int copy) {
+        float most = top;
+#pragma unroll
+        for (int i = 1; i < kSplit; ++i) most = fmaxf(most, hand.value(copy, i, 0));
+        const float used = most == -__builtin_inff() ? 0.0f : most;  // a row without keys
+        const float f = __builtin_amdgcn_exp2f((top - used) * unit);
+        total *= f;
+#pragma unroll
+        for (int d = 0; d < kOut; ++d) acc[d] *= f;
+#pragma unroll
+        for (int i = 1; i < kSplit; ++i) {
+            const float e = __builtin_amdgcn_exp2f((hand.value(copy, i, 0) - used) * unit);
+            total = __builtin_fmaf(hand.value(copy, i, 1), e, total);
+#pragma unroll
+            for (int v = 0; v < 4 * kOut; ++v)
+                acc[v >> 2][v & 3] = __builtin_fmaf(hand.value(copy, i, 2 + v), e, acc[v >> 2][v & 3]);
+        }
+        if (me.row0 >= a.N) return;
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        const int64_t at = heads_row<D>(a, b, h);
+        T *to = static_cast<T*>(a.out) + at, *to_lo = static_cast<T*>(a.out_lo) + at;
+#pragma unroll
+        for (int d = 0; d < kOut; ++d) {
+            const uint32_t lane_at = static_cast<uint32_t>(q) * (a.H * D) + 16 * d + 4 * g;
+            const f32x4 out = acc[d] * inv;
+            const X4 hi = round4<T>(out);
+            *reinterpret_cast<X4*>(to + lane_at) = hi;
+            if (a.out_lo != nullptr) *reinterpret_cast<X4*>(to_lo + lane_at) = round4<T>(out - wide4<T>(hi));
+        }
+        if (g == 0 && a.row_max != nullptr) {
+            const int64_t row = (static_cast<int64_t>(b) * a.H + h) * a.N;
+            (a.row_max + row)[static_cast<uint32_t>(q)] = used;
+            (a.row_inv + row)[static_cast<uint32_t>(q)] = inv;
+        }
+    };
+    wait_vmem();
     __syncthreads();
+    uint32_t before = 0;  // the window before this one
     for (uint32_t i = begin; i < end; ++i) {
         const int buf = (i - begin) & 1;
         const Place here = p;
-        Operand<T, D> qr = qn;
+        const Operand<T, D> qr = qn;
         const bool more = i + 1 < end;
         if (more) {
-            p = place_of<kMask>(a, o, i + 1);
-            kp.load(rows_of<T>(a, p.b, 1, h, D), a.st, a.N);
-            vp.load(rows_of<T>(a, p.b, 2, h, D), a.st, a.N);
-            qn.load(rows_of<T>(a, p.b, 0, h, D) + q * a.st, g);
+            p = places.at(a, o, i + 1);
+            fetch(p.b, buf ^ 1);
         }
-        if (active) {
+        if (me.active) {
+            if (me.leads && i > begin) finish(before, buf ^ 1);
+            before = here.b;
             if (here.kind != kind) {
                 kind = here.kind;
-                build_tiles<NT, kMask, false>(tile, a, h, kind, q, g, side, per_scale);
+                build_tiles<kSpan, kMask, false>(tile, a, h, kind, q, 16 * me.first + 4 * g, side, per_scale);
             }
-            const T *kl = k_lds[buf], *vl = v_lds[buf];
-            const auto score = [&](int t) {
-                Operand<T, D> kr;
-                kr.load_lds(kl, 16 * t, col, g);
-                return multiply<T, D>(kr, qr, kMask ? f32x4{} : tile[t]);
+            const T* vl = v_lds[buf] + me.first * 16 * D;
+            const Halves<T> kl(k_lds[buf] + me.first * 16 * D, 16 * D);
+            // LDS reads run one step ahead of the products on them
+            const auto start = [&](int t) { return kMask ? f32x4{} : tile[t]; };
+            Operand<T, D> kr[2];
+            const auto read = [&](int t) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    if (t + u < kSpan) kr[u].load_lds(kl.of[u], 16 * t, col, g);
             };
-            float top = -__builtin_inff();
+            top = -__builtin_inff();
+            read(0);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const f32x4 s = score(t);
+            for (int t = 0; t < kSpan; t += 2) {
+                f32x4 s[2];
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    top = fmaxf(top, kMask ? __builtin_fmaf(s[r], a.scale, tile[t][r]) : s[r]);
-                if (t % 4 == 3) tiles_in_order();
+                for (int u = 0; u < 2; ++u)
+                    if (t + u < kSpan) s[u] = multiply<T, D>(kr[u], qr, start(t + u));
+                read(t + 2 < kSpan ? t + 2 : 0);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (t + u < kSpan)
+                            top = fmaxf(top, kMask ? __builtin_fmaf(s[u][r], a.scale, tile[t + u][r]) : s[u][r]);
+                }
+                tiles_in_order();
             }
             top = max_groups(top);
-            const float used = top == -__builtin_inff() ? 0.0f : top;  // a row without keys
-            // the scores are computed again below, not kept in registers
-            asm volatile("" : "+v"(qr.v));
-            f32x4 acc[kOut] = {};
-            float total = 0.0f;
+            const float used = top == -__builtin_inff() ? 0.0f : top;
+            // the sum of the weights as one more row of the product
+            f32x4 sum = {};
+#pragma unroll
+            for (int d = 0; d < kOut; ++d) acc[d] = f32x4{};
             const auto weigh = [&](auto large) {
                 const Exponent<kMask, decltype(large)::value> exponent = {a.scale, c2};
                 const float off = used * c2;
 #pragma unroll
-                for (int t = 0; t < NT; t += 2) {
+                for (int t = 0; t < kSpan; t += 2) {
+                    const int count = t + 1 < kSpan ? 2 : 1;
+                    f32x4 s[2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        if (u < count) s[u] = multiply<T, D>(kr[u], qr, start(t + u));
+                    if (t + 2 < kSpan) read(t + 2);
+                    Turned<T, D> vt;
+                    vt.load(vl, 16 * t, count, col, g);
                     X4 hi[2], lo[2];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        f32x4 s = score(t + u);
+                        if (u >= count) continue;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            s[r] = __builtin_amdgcn_exp2f(exponent(s[r], tile[t + u][r], used, 0.0f, off));
-                            total += s[r];
-                        }
-                        settled(total);
-                        hi[u] = round4<T>(s);
-                        lo[u] = round4<T>(s - wide4<T>(hi[u]));
+                        for (int r = 0; r < 4; ++r)
+                            s[u][r] = __builtin_amdgcn_exp2f(exponent(s[u][r], tile[t + u][r], used, 0.0f, off));
+                        split<T>(s[u], hi[u], lo[u]);
                     }
-#pragma unroll
-                    for (int s = 0; s < kOut; ++s) {
-                        const typename Mma<T>::x8 vt = transposed_pair<T, D>(vl, 16 * t, s, col, g);
-                        acc[s] = Mma<T>::mma32(vt, join<T>(hi[0], hi[1]), acc[s]);
-                        acc[s] = Mma<T>::mma32(vt, join<T>(lo[0], lo[1]), acc[s]);
+                    if (count == 2) {
+                        sum = Mma<T>::mma32(join<T>(ones, ones), join<T>(hi[0], hi[1]), sum);
+                        sum = Mma<T>::mma32(join<T>(ones, ones), join<T>(lo[0], lo[1]), sum);
+                    } else {
+                        sum = Mma<T>::mma16(ones, hi[0], sum);
+                        sum = Mma<T>::mma16(ones, lo[0], sum);
                     }
+                    vt.add(acc, count, hi);
+                    vt.add(acc, count, lo);
                     tiles_in_order();
                 }
             };
@@ -356,300 +572,386 @@ __global__ void __launch_bounds__(W * 64) attn_forward_tuned_kernel(const AttnAr
                 weigh(std::true_type{});
             else
                 weigh(std::false_type{});
-            total = sum_groups(total);
-            if (q0 < a.N) {
-                const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-                const int64_t at = ((static_cast<int64_t>(here.b) * a.N + q) * a.H + h) * D;
+            total = sum[0];
+            if (kSplit > 1 && !me.leads) {
+                hand.value(buf, me.part, 0) = top;
+                hand.value(buf, me.part, 1) = total;
 #pragma unroll
-                for (int s = 0; s < kOut; ++s) {
-                    const f32x4 out = acc[s] * inv;
-                    const X4 hi = round4<T>(out);
-                    *reinterpret_cast<X4*>(static_cast<T*>(a.out) + at + 16 * s + 4 * g) = hi;
-                    if (a.out_lo != nullptr)
-                        *reinterpret_cast<X4*>(static_cast<T*>(a.out_lo) + at + 16 * s + 4 * g) =
-                            round4<T>(out - wide4<T>(hi));
-                }
-                if (g == 0 && a.row_max != nullptr) {
-                    const int64_t row = (static_cast<int64_t>(here.b) * a.H + h) * a.N + q;
-                    a.row_max[row] = used;
-                    a.row_inv[row] = inv;
-                }
+                for (int v = 0; v < 4 * kOut; ++v) hand.value(buf, me.part, 2 + v) = acc[v >> 2][v & 3];
             }
         }
-        if (more) {
-            kp.store(k_lds[buf ^ 1]);
-            vp.store(v_lds[buf ^ 1]);
-            __syncthreads();
-        }
+        wait_vmem();
+        __syncthreads();
     }
+    if (me.active && me.leads && end > begin) finish(before, (end - 1 - begin) & 1);
 }
 
 // dq, delta and a range's share of dbias.
-template <typename T, int D, int NT, int W, bool kMask>
-__global__ void __launch_bounds__(W * 64) attn_grad_q_tuned_kernel(const AttnArgs a, const Order o, const Walk w) {
+template <typename T, int D, int NT, int S, int kSplit, int kWaves, bool kMask>
+__global__ void __launch_bounds__(S* kSplit * 64) __attribute__((amdgpu_waves_per_eu(kWaves)))
+attn_grad_q_tuned_kernel(const AttnArgs a, const Order o, const Walk w) {
     typedef typename Mma<T>::x4 X4;
-    constexpr int kTile = NT * 16 * D;
-    constexpr int kOut = D / 16;
+    typedef Share<NT, S, kSplit> Mine;
+    constexpr int kTile = NT * 16 * D, W = S * kSplit, kOut = D / 16, kSpan = Mine::kSpan;
+    typedef Handover<S, kSplit, 4 * kOut> Hand;
     __shared__ __attribute__((aligned(16))) T k_lds[2][kTile];
     __shared__ __attribute__((aligned(16))) T v_lds[2][kTile];
+    __shared__ float hand_lds[Hand::kFloats];
     __shared__ uint8_t side[kMask ? 4 : NT * 16];
     uint32_t range, group;
     int h;
     if (!walk_of(a, w, range, group, h)) return;
     const uint32_t begin = range * w.per, end = std::min(a.B, begin + w.per);
-    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-    const int strip = static_cast<int>(group) * W + (threadIdx.x >> 6);
-    const int q0 = strip * 16 + col, q = q0 < a.N ? q0 : a.N - 1;
-    const bool active = strip * 16 < a.N;
+    const Mine me(a, group);
+    const int col = me.col, g = me.g, q = me.row;
+    const Hand hand(hand_lds, me.local, me.lane);
     const float per_scale = 1.0f / a.scale, c2 = a.scale * kLog2e;
     if constexpr (!kMask) token_sides(a, side, std::min(a.N, NT * 16));
-    f32x4 tile[NT], sums[NT] = {};
+    f32x4 tile[kSpan], sums[kSpan] = {};
     uint32_t kind = ~0u;
-    Pieces<T, D, NT, W> pieces;
-    Operand<T, D> qn, gn;
-    const auto fetch_rows = [&](uint32_t b) {
-        qn.load(rows_of<T>(a, b, 0, h, D) + q * a.st, g);
-        gn.load(static_cast<const T*>(a.grad_out) + ((static_cast<int64_t>(b) * a.N + q) * a.H + h) * D, g);
+    // the window ahead: the lane's rows and their statistics
+    Operand<T, D> qn, gn, out_n, rest_n;
+    float top_n, inv_n;
+    const Rows<T, D, NT, W> rows(static_cast<uint32_t>(a.st), a.N);
+    const uint32_t mine = static_cast<uint32_t>(q) * static_cast<uint32_t>(a.st);
+    const uint32_t mine_out = static_cast<uint32_t>(q) * (a.H * D);
+    const auto fetch = [&](uint32_t b, int buf) {
+        rows.load(rows_of<T>(a, b, 1, h, D), lds_address(k_lds[0]) + buf * kTile * sizeof(T));
+        rows.load(rows_of<T>(a, b, 2, h, D), lds_address(v_lds[0]) + buf * kTile * sizeof(T));
+        qn.load(rows_of<T>(a, b, 0, h, D), mine, g);
+        const int64_t row = (static_cast<int64_t>(b) * a.H + h) * a.N, at = heads_row<D>(a, b, h);
+        gn.load(static_cast<const T*>(a.grad_out) + at, mine_out, g);
+        out_n.load(static_cast<const T*>(a.out) + at, mine_out, g);
+        rest_n.load(static_cast<const T*>(a.out_lo) + at, mine_out, g);
+        top_n = (a.row_max + row)[static_cast<uint32_t>(q)];
+        inv_n = (a.row_inv + row)[static_cast<uint32_t>(q)];
     };
-    Place p = place_of<kMask>(a, o, begin);
-    pieces.load(rows_of<T>(a, p.b, 1, h, D), a.st, a.N);
-    fetch_rows(p.b);
-    pieces.store(k_lds[0]);
-    pieces.load(rows_of<T>(a, p.b, 2, h, D), a.st, a.N);
-    pieces.store(v_lds[0]);
+    Places<kMask> places(begin, end);
+    Place p = places.at(a, o, begin);
+    fetch(p.b, 0);
+    f32x4 acc[kOut];
+    const auto finish = [&](uint32_t b, int copy) {
+#pragma unroll
+        for (int i = 1; i < kSplit; ++i) {
+#pragma unroll
+            for (int v = 0; v < 4 * kOut; ++v) acc[v >> 2][v & 3] += hand.value(copy, i, v);
+        }
+        if (me.row0 >= a.N) return;
+        T* to = static_cast<T*>(a.grad_qkv) + (static_cast<int64_t>(b) * a.N * 3 * a.H + h) * D;
+#pragma unroll
+        for (int d = 0; d < kOut; ++d)
+            *reinterpret_cast<X4*>(to + (3 * mine_out + 16 * d + 4 * g)) = round4<T>(acc[d] * a.scale);
+    };
+    wait_vmem();
     __syncthreads();
+    uint32_t before = 0;
     for (uint32_t i = begin; i < end; ++i) {
         const int buf = (i - begin) & 1;
         const Place here = p;
         const Operand<T, D> qr = qn, go = gn;
         const bool more = i + 1 < end;
-        // the row's statistics and output, then the next window's rows
-        const int64_t row = (static_cast<int64_t>(here.b) * a.H + h) * a.N + q;
-        const int64_t at = ((static_cast<int64_t>(here.b) * a.N + q) * a.H + h) * D;
-        Operand<T, D> out, rest;
-        out.load(static_cast<const T*>(a.out) + at, g);
-        rest.load(static_cast<const T*>(a.out_lo) + at, g);
-        const float top = a.row_max[row], inv = a.row_inv[row];
+        const Operand<T, D> out = out_n, rest = rest_n;
+        const float top = top_n, inv = inv_n;
         if (more) {
-            p = place_of<kMask>(a, o, i + 1);
-            pieces.load(rows_of<T>(a, p.b, 1, h, D), a.st, a.N);
-            fetch_rows(p.b);
+            p = places.at(a, o, i + 1);
+            fetch(p.b, buf ^ 1);
         }
-        float delta = 0.0f;
-#pragma unroll
-        for (int e = 0; e < D / 4; ++e) delta = __builtin_fmaf(out.dim(e) + rest.dim(e), go.dim(e), delta);
-        delta = sum_groups(delta);
-        f32x4 acc[kOut] = {};
-        const auto half = [&](auto large, int from, int to) {
-            const Exponent<kMask, decltype(large)::value> exponent = {a.scale, c2};
-            const float plus = __builtin_amdgcn_logf(inv), off = top * c2 - plus;
-            const T *kl = k_lds[buf], *vl = v_lds[buf];
-#pragma unroll
-            for (int t = 0; t < NT; t += 2) {
-                if (t < from || t >= to) continue;
-                X4 ds[2];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    Operand<T, D> kr, vr;
-                    kr.load_lds(kl, 16 * (t + u), col, g);
-                    vr.load_lds(vl, 16 * (t + u), col, g);
-                    f32x4 s = multiply<T, D>(kr, qr, kMask ? f32x4{} : tile[t + u]);
-                    const f32x4 dp = multiply<T, D>(vr, go, f32x4{-delta, -delta, -delta, -delta});
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        s[r] = __builtin_amdgcn_exp2f(exponent(s[r], tile[t + u][r], top, plus, off)) * dp[r];
-                        sums[t + u][r] += s[r];
-                    }
-                    settled(sums[t + u]);
-                    ds[u] = round4<T>(s);
-                }
-#pragma unroll
-                for (int s = 0; s < kOut; ++s)
-                    acc[s] = Mma<T>::mma32(transposed_pair<T, D>(kl, 16 * t, s, col, g), join<T>(ds[0], ds[1]), acc[s]);
-                tiles_in_order();
-            }
-        };
-        constexpr int kHalf = NT / 4 * 2;
-        const bool large = !kMask && __any(fabsf(top * c2) > kLargeLog2);
-        if (active) {
+        if (me.active) {
+            if (me.leads && i > begin) finish(before, buf ^ 1);
+            before = here.b;
             if (here.kind != kind) {
                 kind = here.kind;
-                build_tiles<NT, kMask, false>(tile, a, h, kind, q, g, side, per_scale);
+                build_tiles<kSpan, kMask, false>(tile, a, h, kind, q, 16 * me.first + 4 * g, side, per_scale);
             }
-            half(std::true_type{}, 0, kHalf);
-        }
-        if (more) {
-            pieces.store(k_lds[buf ^ 1]);
-            pieces.load(rows_of<T>(a, p.b, 2, h, D), a.st, a.N);
-        }
-        if (active) {
-            half(std::true_type{}, kHalf, NT);
-            if (q0 < a.N) {
-                T* to = static_cast<T*>(a.grad_qkv) + ((static_cast<int64_t>(here.b) * a.N + q) * 3 * a.H + h) * D;
+            float delta = 0.0f;
 #pragma unroll
-                for (int s = 0; s < kOut; ++s)
-                    *reinterpret_cast<X4*>(to + 16 * s + 4 * g) = round4<T>(acc[s] * a.scale);
-                if (g == 0) a.delta[row] = delta;
+            for (int e = 0; e < D / 4; ++e) delta = __builtin_fmaf(out.dim(e) + rest.dim(e), go.dim(e), delta);
+            delta = sum_groups(delta);
+            if (me.leads && g == 0 && me.row0 < a.N)
+                (a.delta + (static_cast<int64_t>(here.b) * a.H + h) * a.N)[static_cast<uint32_t>(q)] = delta;
+            const float plus = __builtin_amdgcn_logf(inv), off = top * c2 - plus;
+#pragma unroll
+            for (int d = 0; d < kOut; ++d) acc[d] = f32x4{};
+            const T* kt = k_lds[buf] + me.first * 16 * D;
+            const Halves<T> kl(kt, 16 * D), vl(v_lds[buf] + me.first * 16 * D, 16 * D);
+            const auto walk = [&](auto large) {
+                const Exponent<kMask, decltype(large)::value> exponent = {a.scale, c2};
+                Operand<T, D> kr[2], vr[2];
+                const auto read = [&](int t) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        if (t + u >= kSpan) continue;
+                        kr[u].load_lds(kl.of[u], 16 * t, col, g);
+                        vr[u].load_lds(vl.of[u], 16 * t, col, g);
+                    }
+                };
+                read(0);
+#pragma unroll
+                for (int t = 0; t < kSpan; t += 2) {
+                    const int count = t + 1 < kSpan ? 2 : 1;
+                    f32x4 s[2], dp[2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        if (u >= count) continue;
+                        s[u] = multiply<T, D>(kr[u], qr, kMask ? f32x4{} : tile[t + u]);
+                        dp[u] = multiply<T, D>(vr[u], go, f32x4{-delta, -delta, -delta, -delta});
+                    }
+                    if (t + 2 < kSpan) read(t + 2);
+                    Turned<T, D> k_turned;
+                    k_turned.load(kt, 16 * t, count, col, g);
+                    X4 ds[2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        if (u >= count) continue;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            s[u][r] = __builtin_amdgcn_exp2f(exponent(s[u][r], tile[t + u][r], top, plus, off)) * dp[u][r];
+                            sums[t + u][r] += s[u][r];
+                        }
+                        settled(sums[t + u]);
+                        ds[u] = round4<T>(s[u]);
+                    }
+                    k_turned.add(acc, count, ds);
+                    tiles_in_order();
+                }
+            };
+            if (!kMask && __any(fabsf(top * c2) > kLargeLog2))
+                walk(std::true_type{});
+            else
+                walk(std::false_type{});
+            if (kSplit > 1 && !me.leads) {
+#pragma unroll
+                for (int v = 0; v < 4 * kOut; ++v) hand.value(buf, me.part, v) = acc[v >> 2][v & 3];
             }
         }
-        if (more) {
-            pieces.store(v_lds[buf ^ 1]);
-            __syncthreads();
-        }
+        wait_vmem();
+        __syncthreads();
     }
-    if (!active || q0 >= a.N || a.grad_bias == nullptr) return;
+    if (!me.active) return;
+    if (me.leads && end > begin) finish(before, (end - 1 - begin) & 1);
+    if (me.row0 >= a.N || a.grad_bias == nullptr) return;
     float* to = a.grad_bias + ((static_cast<int64_t>(range) * a.H + h) * a.N + q) * a.N;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    for (int t = 0; t < kSpan; ++t) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int k = 16 * t + 4 * g + r;
+            const int k = 16 * (me.first + t) + 4 * g + r;
             if (k < a.N) to[k] = sums[t][r];
         }
     }
 }
 
-// dk and dv: a wave owns 16 keys.
-template <typename T, int D, int NT, int W, bool kMask>
-__global__ void __launch_bounds__(W * 64) attn_grad_kv_tuned_kernel(const AttnArgs a, const Order o, const Walk w) {
+// dk and dv: a strip is 16 keys, the other axis the queries.
+template <typename T, int D, int NT, int S, int kSplit, int kWaves, bool kMask>
+__global__ void __launch_bounds__(S* kSplit * 64) __attribute__((amdgpu_waves_per_eu(kWaves)))
+attn_grad_kv_tuned_kernel(const AttnArgs a, const Order o, const Walk w) {
     typedef typename Mma<T>::x4 X4;
-    constexpr int kTile = NT * 16 * D, kRows = NT * 16, kEach = (kRows + W * 64 - 1) / (W * 64);
-    constexpr int kOut = D / 16;
+    typedef Share<NT, S, kSplit> Mine;
+    constexpr int kTile = NT * 16 * D, W = S * kSplit, kOut = D / 16, kSpan = Mine::kSpan;
+    constexpr int kRows = NT * 16, kEach = (kRows + W * 64 - 1) / (W * 64);
+    typedef Handover<S, kSplit, 8 * kOut> Hand;
     __shared__ __attribute__((aligned(16))) T q_lds[2][kTile];
     __shared__ __attribute__((aligned(16))) T o_lds[2][kTile];
-    // per query: largest score, log2 of 1 / sum, -delta
-    __shared__ __attribute__((aligned(16))) float top_lds[2][kRows], plus_lds[2][kRows], delta_lds[2][kRows];
+    __shared__ float hand_lds[Hand::kFloats];
+    // per query: largest score and log2 of 1 / sum (lse: both as one, in units
+    // of the accumulator), delta; per wave: whether it saw a large score
+    __shared__ float top_lds[2][kRows], plus_lds[2][kRows], lse_lds[kMask ? 1 : 2][kRows], delta_lds[2][kRows];
+    __shared__ uint32_t large_lds[2][W];
     __shared__ uint8_t side[kMask ? 4 : kRows];
     uint32_t range, group;
     int h;
     if (!walk_of(a, w, range, group, h)) return;
     const uint32_t begin = range * w.per, end = std::min(a.B, begin + w.per);
-    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-    const int strip = static_cast<int>(group) * W + (threadIdx.x >> 6);
-    const int k0 = strip * 16 + col, k = k0 < a.N ? k0 : a.N - 1;
-    const bool active = strip * 16 < a.N;
+    const Mine me(a, group);
+    const int col = me.col, g = me.g, k = me.row;
+    const Hand hand(hand_lds, me.local, me.lane);
     const float per_scale = 1.0f / a.scale, c2 = a.scale * kLog2e;
     if constexpr (!kMask) token_sides(a, side, std::min(a.N, kRows));
-    f32x4 tile[NT];
+    f32x4 tile[kSpan];
     uint32_t kind = ~0u;
-    Pieces<T, D, NT, W> qp, op;
-    float top_r[kEach], plus_r[kEach], delta_r[kEach];
+    float top_r[kEach], inv_r[kEach], delta_r[kEach];
     Operand<T, D> kn, vn;
-    const auto fetch = [&](uint32_t b) {
-        const T* first = static_cast<const T*>(a.grad_out) + (static_cast<int64_t>(b) * a.N * a.H + h) * D;
-        qp.load(rows_of<T>(a, b, 0, h, D), a.st, a.N);
-        op.load(first, static_cast<int64_t>(a.H) * D, a.N);
-        kn.load(rows_of<T>(a, b, 1, h, D) + k * a.st, g);
-        vn.load(rows_of<T>(a, b, 2, h, D) + k * a.st, g);
+    const Rows<T, D, NT, W> rows(static_cast<uint32_t>(a.st), a.N), out_rows(static_cast<uint32_t>(a.H * D), a.N);
+    const uint32_t mine = static_cast<uint32_t>(k) * static_cast<uint32_t>(a.st);
+    const auto fetch = [&](uint32_t b, int buf) {
+        rows.load(rows_of<T>(a, b, 0, h, D), lds_address(q_lds[0]) + buf * kTile * sizeof(T));
+        out_rows.load(static_cast<const T*>(a.grad_out) + heads_row<D>(a, b, h),
+                      lds_address(o_lds[0]) + buf * kTile * sizeof(T));
+        kn.load(rows_of<T>(a, b, 1, h, D), mine, g);
+        vn.load(rows_of<T>(a, b, 2, h, D), mine, g);
         const int64_t row = (static_cast<int64_t>(b) * a.H + h) * a.N;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             const int r = threadIdx.x + i * W * 64;
             const bool in = r < a.N;
-            const int64_t at = row + (in ? r : a.N - 1);
-            top_r[i] = in ? a.row_max[at] : 0.0f;
-            plus_r[i] = in ? a.row_inv[at] : 0.0f;  // queries past N: log2 0 = -inf, no weight
-            delta_r[i] = in ? a.delta[at] : 0.0f;
+            const uint32_t at = in ? r : a.N - 1;
+            top_r[i] = in ? (a.row_max + row)[at] : 0.0f;
+            inv_r[i] = in ? (a.row_inv + row)[at] : 0.0f;  // queries past N: log2 0 = -inf, no weight
+            delta_r[i] = in ? (a.delta + row)[at] : 0.0f;
         }
     };
     const auto keep = [&](int buf) {
-        qp.store(q_lds[buf]);
-        op.store(o_lds[buf]);
+        bool large = false;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             const int r = threadIdx.x + i * W * 64;
             if (r >= kRows) break;
+            const float plus = __builtin_amdgcn_logf(inv_r[i]);
             top_lds[buf][r] = top_r[i];
-            plus_lds[buf][r] = __builtin_amdgcn_logf(plus_r[i]);
-            delta_lds[buf][r] = -delta_r[i];
+            plus_lds[buf][r] = plus;
+            if constexpr (!kMask) lse_lds[buf][r] = top_r[i] - plus * (1.0f / c2);
+            delta_lds[buf][r] = delta_r[i];
+            large = large || fabsf(top_r[i] * c2) > kLargeLog2;
+        }
+        if constexpr (!kMask) {
+            large = __any(large);
+            if (me.lane == 0) large_lds[buf][threadIdx.x >> 6] = large ? 1 : 0;
         }
     };
-    Place p = place_of<kMask>(a, o, begin);
-    fetch(p.b);
+    Places<kMask> places(begin, end);
+    Place p = places.at(a, o, begin);
+    fetch(p.b, 0);
     keep(0);
+    f32x4 dk[kOut], dv[kOut];
+    const auto finish = [&](uint32_t b, int copy) {
+#pragma unroll
+        for (int i = 1; i < kSplit; ++i) {
+#pragma unroll
+            for (int v = 0; v < 4 * kOut; ++v) {
+                dk[v >> 2][v & 3] += hand.value(copy, i, v);
+                dv[v >> 2][v & 3] += hand.value(copy, i, 4 * kOut + v);
+            }
+        }
+        if (me.row0 >= a.N) return;
+        const uint32_t hd = static_cast<uint32_t>(a.H * D);
+        T* to = static_cast<T*>(a.grad_qkv) + (static_cast<int64_t>(b) * a.N * 3 * a.H + a.H + h) * D;
+#pragma unroll
+        for (int d = 0; d < kOut; ++d) {
+            const uint32_t at = 3 * hd * static_cast<uint32_t>(k) + 16 * d + 4 * g;
+            *reinterpret_cast<X4*>(to + at) = round4<T>(dk[d] * a.scale);
+            *reinterpret_cast<X4*>(to + hd + at) = round4<T>(dv[d]);
+        }
+    };
+    wait_vmem();
     __syncthreads();
+    uint32_t before = 0;
     for (uint32_t i = begin; i < end; ++i) {
         const int buf = (i - begin) & 1;
         const Place here = p;
         const Operand<T, D> kr = kn, vr = vn;
         const bool more = i + 1 < end;
         if (more) {
-            p = place_of<kMask>(a, o, i + 1);
-            fetch(p.b);
+            p = places.at(a, o, i + 1);
+            fetch(p.b, buf ^ 1);
         }
-        if (active) {
+        if (me.active) {
+            if (me.leads && i > begin) finish(before, buf ^ 1);
+            before = here.b;
             if (here.kind != kind) {
                 kind = here.kind;
-                build_tiles<NT, kMask, true>(tile, a, h, kind, k, g, side, per_scale);
+                build_tiles<kSpan, kMask, true>(tile, a, h, kind, k, 16 * me.first + 4 * g, side, per_scale);
             }
-            const T *ql = q_lds[buf], *ol = o_lds[buf];
-            const Exponent<kMask, true> exponent = {a.scale, c2};
-            f32x4 dk[kOut] = {}, dv[kOut] = {};
+            const T *qt = q_lds[buf] + me.first * 16 * D, *ot = o_lds[buf] + me.first * 16 * D;
+            const Halves<T> ql(qt, 16 * D), ol(ot, 16 * D);
+            const int stat = 16 * me.first + 4 * g + (col & 3);
 #pragma unroll
-            for (int t = 0; t < NT; t += 2) {
-                X4 pw[2], ds[2];
+            for (int d = 0; d < kOut; ++d) dk[d] = dv[d] = f32x4{};
+            const auto walk = [&](auto large) {
+                // with a mask tensor, and with large scores, top and plus apart
+                constexpr bool kApart = kMask || decltype(large)::value;
+                const Exponent<kMask, true> exponent = {a.scale, c2};
+                Operand<T, D> qr[2], go[2];
+                float top[2], plus[2], delta[2];
+                // a lane holds the statistics of query 4 g + col % 4 of a tile
+                const auto read = [&](int t) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int first = 16 * (t + u) + 4 * g;
-                    Operand<T, D> qr, go;
-                    qr.load_lds(ql, 16 * (t + u), col, g);
-                    go.load_lds(ol, 16 * (t + u), col, g);
-                    const f32x4 top = *reinterpret_cast<const f32x4*>(&top_lds[buf][first]);
-                    const f32x4 plus = *reinterpret_cast<const f32x4*>(&plus_lds[buf][first]);
-                    const f32x4 delta = *reinterpret_cast<const f32x4*>(&delta_lds[buf][first]);
-                    f32x4 s = multiply<T, D>(qr, kr, kMask ? f32x4{} : tile[t + u]);
-                    f32x4 dp = multiply<T, D>(go, vr, delta);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        s[r] = __builtin_amdgcn_exp2f(exponent(s[r], tile[t + u][r], top[r], plus[r], 0.0f));
-                        dp[r] *= s[r];
+                    for (int u = 0; u < 2; ++u) {
+                        if (t + u >= kSpan) continue;
+                        const int at = stat + 16 * (t + u);
+                        qr[u].load_lds(ql.of[u], 16 * t, col, g);
+                        go[u].load_lds(ol.of[u], 16 * t, col, g);
+                        top[u] = kApart ? top_lds[buf][at] : lse_lds[kMask ? 0 : buf][at];
+                        if (kApart) plus[u] = plus_lds[buf][at];
+                        delta[u] = delta_lds[buf][at];
                     }
-                    pw[u] = round4<T>(s);
-                    ds[u] = round4<T>(dp);
-                }
+                };
+                read(0);
 #pragma unroll
-                for (int s = 0; s < kOut; ++s) {
-                    dv[s] = Mma<T>::mma32(transposed_pair<T, D>(ol, 16 * t, s, col, g), join<T>(pw[0], pw[1]), dv[s]);
-                    dk[s] = Mma<T>::mma32(transposed_pair<T, D>(ql, 16 * t, s, col, g), join<T>(ds[0], ds[1]), dk[s]);
-                }
-                tiles_in_order();
-            }
-            if (k0 < a.N) {
-                const int64_t hd = static_cast<int64_t>(a.H) * D;
-                T* to = static_cast<T*>(a.grad_qkv) + ((static_cast<int64_t>(here.b) * a.N + k) * 3 * a.H + h) * D + hd;
+                for (int t = 0; t < kSpan; t += 2) {
+                    const int count = t + 1 < kSpan ? 2 : 1;
+                    f32x4 s[2], dp[2];
+                    float top_t[2], plus_t[2], delta_t[2];
 #pragma unroll
-                for (int s = 0; s < kOut; ++s) {
-                    *reinterpret_cast<X4*>(to + 16 * s + 4 * g) = round4<T>(dk[s] * a.scale);
-                    *reinterpret_cast<X4*>(to + hd + 16 * s + 4 * g) = round4<T>(dv[s]);
+                    for (int u = 0; u < 2; ++u) {
+                        if (u >= count) continue;
+                        s[u] = multiply<T, D>(qr[u], kr, kMask ? f32x4{} : tile[t + u]);
+                        dp[u] = multiply<T, D>(go[u], vr, f32x4{});
+                        top_t[u] = top[u], delta_t[u] = delta[u];
+                        if (kApart) plus_t[u] = plus[u];
+                    }
+                    if (t + 2 < kSpan) read(t + 2);
+                    Turned<T, D> o_turned, q_turned;
+                    o_turned.load(ot, 16 * t, count, col, g);
+                    q_turned.load(qt, 16 * t, count, col, g);
+                    X4 pw[2], ds[2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        if (u >= count) continue;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float e = kApart ? exponent(s[u][r], tile[t + u][r], of_row(top_t[u], r),
+                                                              of_row(plus_t[u], r), 0.0f)
+                                                   : (s[u][r] - of_row(top_t[u], r)) * c2;
+                            s[u][r] = __builtin_amdgcn_exp2f(e);
+                            dp[u][r] = (dp[u][r] - of_row(delta_t[u], r)) * s[u][r];
+                        }
+                        pw[u] = round4<T>(s[u]);
+                        ds[u] = round4<T>(dp[u]);
+                    }
+                    o_turned.add(dv, count, pw);
+                    q_turned.add(dk, count, ds);
+                    tiles_in_order();
+                }
+            };
+            if (!kMask && __any(me.lane < W && large_lds[buf][me.lane < W ? me.lane : 0] != 0))
+                walk(std::true_type{});
+            else
+                walk(std::false_type{});
+            if (kSplit > 1 && !me.leads) {
+#pragma unroll
+                for (int v = 0; v < 4 * kOut; ++v) {
+                    hand.value(buf, me.part, v) = dk[v >> 2][v & 3];
+                    hand.value(buf, me.part, 4 * kOut + v) = dv[v >> 2][v & 3];
                 }
             }
         }
-        if (more) {
-            keep(buf ^ 1);
-            __syncthreads();
-        }
+        if (more) keep(buf ^ 1);
+        wait_vmem();
+        __syncthreads();
     }
+    if (me.active && me.leads && end > begin) finish(before, (end - 1 - begin) & 1);
 }
 
 // ---- launchers ------------------------------------------------------------------
 
 template <typename T, int D, int NT, bool kMask>
 void launch_forward(const AttnArgs& a, const Order& o, hipStream_t s) {
-    constexpr int W = tuned_waves(NT, kForwardPass);
-    const Walk w = tuned_walk(a.B, a.H, a.N, kForwardPass);
+    constexpr Form f = tuned_form(NT, D, kForwardPass);
+    const Walk w = tuned_walk(a.B, a.H, a.N, D, kForwardPass);
     const uint32_t grid = xcd_launch_count(w.groups * static_cast<uint32_t>(a.H) * w.ranges);
-    attn_forward_tuned_kernel<T, D, NT, W, kMask><<<grid, W * 64, 0, s>>>(a, o, w);
+    attn_forward_tuned_kernel<T, D, NT, f.strips, f.split, f.per_simd, kMask>
+        <<<grid, f.strips * f.split * 64, 0, s>>>(a, o, w);
 }
 
 template <typename T, int D, int NT, bool kMask>
 void launch_backward(const AttnArgs& a, const Order& o, hipStream_t s) {
-    constexpr int W = tuned_waves(NT, kQueryPass), V = tuned_waves(NT, kKeyPass);
-    const Walk w = tuned_walk(a.B, a.H, a.N, kQueryPass), v = tuned_walk(a.B, a.H, a.N, kKeyPass);
+    constexpr Form f = tuned_form(NT, D, kQueryPass), e = tuned_form(NT, D, kKeyPass);
+    const Walk w = tuned_walk(a.B, a.H, a.N, D, kQueryPass), v = tuned_walk(a.B, a.H, a.N, D, kKeyPass);
     const uint32_t heads = static_cast<uint32_t>(a.H);
-    attn_grad_q_tuned_kernel<T, D, NT, W, kMask>
-        <<<xcd_launch_count(w.groups * heads * w.ranges), W * 64, 0, s>>>(a, o, w);
-    attn_grad_kv_tuned_kernel<T, D, NT, V, kMask>
-        <<<xcd_launch_count(v.groups * heads * v.ranges), V * 64, 0, s>>>(a, o, v);
+    attn_grad_q_tuned_kernel<T, D, NT, f.strips, f.split, f.per_simd, kMask>
+        <<<xcd_launch_count(w.groups * heads * w.ranges), f.strips * f.split * 64, 0, s>>>(a, o, w);
+    attn_grad_kv_tuned_kernel<T, D, NT, e.strips, e.split, e.per_simd, kMask>
+        <<<xcd_launch_count(v.groups * heads * v.ranges), e.strips * e.split * 64, 0, s>>>(a, o, v);
 }
 
 template <typename T, int D, bool kMask>

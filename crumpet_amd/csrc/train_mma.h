@@ -99,6 +99,40 @@ __device__ __forceinline__ typename Mma<T>::x4 load_transposed(const T* tile, in
     }
 }
 
+// 16 bytes per lane from a buffer straight into LDS, at lds_addr + 16 * lane
+// (lds_addr the same for the wave).  Inline asm, so that the compiler does not
+// wait for it before unrelated LDS reads; the caller waits (wait_vmem) before
+// the barrier that publishes the rows.  M0 is an operand, so the compiler
+// writes it; the wait states are those that the load needs after scalar writes
+// of M0 and vector writes of the descriptor's registers, which the compiler
+// does not insert around asm.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void load_to_lds(u32x4 buffer, uint32_t lds_addr, uint32_t offset) {
+    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                 :
+                 : "v"(offset), "s"(buffer), "{m0}"(lds_addr)
+                 : "memory");
+}
+// All vector memory of the wave is done, what the compiler does not see too.
+__device__ __forceinline__ void wait_vmem() {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0) expcnt(7) lgkmcnt(15)
+}
+// A buffer of `bytes` from `first`, the same for the wave.
+__device__ __forceinline__ u32x4 buffer_of(const void* first, uint32_t bytes) {
+    const uint64_t at = reinterpret_cast<uintptr_t>(first);
+    u32x4 b;
+    b[0] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at));
+    b[1] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at >> 32) & 0xffffu);
+    b[2] = __builtin_amdgcn_readfirstlane(bytes);
+    b[3] = 0x00020000;
+    return b;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t lds_address(const T* p) {
+    typedef __attribute__((address_space(3))) const T LdsT;
+    return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsT*)p)));
+}
+
 // Over the 4 lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48).
 __device__ __forceinline__ float sum_groups(float x) {
     x += __shfl_xor(x, 16);
