@@ -54,6 +54,12 @@ __device__ __forceinline__ uint32_t token_class(const Region& r, uint32_t seam, 
     return past & seam;
 }
 
+// Four neighbours at any address: one wide load, at any alignment of an element.
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Four {
+    T v[4];
+};
+
 // What one (window, head) adds to a score.
 struct Terms {
     const float* bias;   // [N, N] of the head
@@ -66,13 +72,56 @@ struct Terms {
         if (a.mode == kTensorMask) mask_at = static_cast<int64_t>(b % a.mask_batch) * a.mask_sb;
         if (a.mode == kRegionMask) seam = seams(a.region, b);
     }
-    // q and k inside the window; their region classes
-    __device__ __forceinline__ float score(const AttnArgs& a, float qk, int q, int k, uint32_t cq, uint32_t ck) const {
+    // Scores of query q and keys k .. k + 3; keys past N are -inf.  cls: the
+    // region classes of the keys.
+    __device__ __forceinline__ f32x4 of_query(const AttnArgs& a, f32x4 qk, int q, int k, uint32_t cq,
+                                              const uint32_t* cls) const {
         const int64_t at = static_cast<int64_t>(q) * a.N + k;
-        float s = __builtin_fmaf(qk, a.scale, bias[at]);
-        if (a.mode == kTensorMask) s += load_float(mask, a.mask_dtype, mask_at + at);
-        if (cq != ck) s -= 100.0f;
+        f32x4 s;
+        if (k + 4 <= a.N) {
+            const Four<float> b = *reinterpret_cast<const Four<float>*>(bias + at);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[r] = __builtin_fmaf(qk[r], a.scale, b.v[r]);
+            if (a.mode == kTensorMask) {
+                if (a.mask_dtype == CRUMPET_DTYPE_F32) add<float>(s, at);
+                else if (a.mask_dtype == CRUMPET_DTYPE_F16) add<_Float16>(s, at);
+                else add<__bf16>(s, at);
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[r] = -__builtin_inff();
+                if (k + r >= a.N) continue;
+                s[r] = __builtin_fmaf(qk[r], a.scale, bias[at + r]);
+                if (a.mode == kTensorMask) s[r] += load_float(mask, a.mask_dtype, mask_at + at + r);
+            }
+        }
+        if (seam) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[r] -= cq != cls[r] ? 100.0f : 0.0f;
+        }
         return s;
+    }
+    // Scores of queries q .. q + 3 and key k; rows past N are anything.
+    __device__ __forceinline__ f32x4 of_key(const AttnArgs& a, f32x4 qk, int q, int k, const uint32_t* cls,
+                                            uint32_t ck) const {
+        f32x4 s;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int64_t at = static_cast<int64_t>(q + r < a.N ? q + r : a.N - 1) * a.N + k;
+            s[r] = __builtin_fmaf(qk[r], a.scale, bias[at]);
+            if (a.mode == kTensorMask) s[r] += load_float(mask, a.mask_dtype, mask_at + at);
+            if (seam) s[r] -= ck != cls[r] ? 100.0f : 0.0f;
+        }
+        return s;
+    }
+
+private:
+    template <typename M>
+    __device__ __forceinline__ void add(f32x4& s, int64_t at) const {
+        const Four<M> m = *reinterpret_cast<const Four<M>*>(static_cast<const M*>(mask) + mask_at + at);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] += static_cast<float>(m.v[r]);
     }
 };
 
@@ -165,13 +214,10 @@ __global__ void __launch_bounds__(kThreads) attn_forward_kernel(const AttnArgs a
         float high = top;
 #pragma unroll
         for (int t = 0; t < L::kRows / 16; ++t) {
-            s[t] = product<T, D>(k_lds, 16 * t, qr, col, g);
+            const int i = 16 * t + 4 * g;
+            s[t] = terms.of_query(a, product<T, D>(k_lds, 16 * t, qr, col, g), q, k0 + i, cq, cls + i);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * t + 4 * g + r, k = k0 + i;
-                s[t][r] = k < a.N ? terms.score(a, s[t][r], q, k, cq, cls[i]) : -__builtin_inff();
-                high = fmaxf(high, s[t][r]);
-            }
+            for (int r = 0; r < 4; ++r) high = fmaxf(high, s[t][r]);
         }
         high = max_groups(high);
         // a row without keys so far: exp(-inf - 0) = 0
@@ -271,13 +317,11 @@ __global__ void __launch_bounds__(kThreads) attn_grad_q_kernel(const AttnArgs a,
         __syncthreads();
 #pragma unroll
         for (int t = 0; t < L::kRows / 16; ++t) {
-            f32x4 s = product<T, D>(k_lds, 16 * t, qr, col, g);
+            const int i = 16 * t + 4 * g;
+            f32x4 s = terms.of_query(a, product<T, D>(k_lds, 16 * t, qr, col, g), q, k0 + i, cq, cls + i);
             const f32x4 dp = product<T, D>(v_lds, 16 * t, go, col, g);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * t + 4 * g + r, k = k0 + i;
-                s[r] = k < a.N ? weight(terms.score(a, s[r], q, k, cq, cls[i]), top) * inv * (dp[r] - delta) : 0.0f;
-            }
+            for (int r = 0; r < 4; ++r) s[r] = k0 + i + r < a.N ? weight(s[r], top) * inv * (dp[r] - delta) : 0.0f;
             accumulate<T, D>(acc, k_lds, 16 * t, round4<T>(s), col, g);
         }
     }
@@ -325,13 +369,14 @@ __global__ void __launch_bounds__(kThreads) attn_grad_kv_kernel(const AttnArgs a
         __syncthreads();
 #pragma unroll
         for (int t = 0; t < L::kRows / 16; ++t) {
-            f32x4 p = product<T, D>(q_lds, 16 * t, kr, col, g);
+            const int first = 16 * t + 4 * g;
+            f32x4 p = terms.of_key(a, product<T, D>(q_lds, 16 * t, kr, col, g), q0 + first, k, cls + first, ck);
             f32x4 ds = product<T, D>(o_lds, 16 * t, vr, col, g);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int i = 16 * t + 4 * g + r, q = q0 + i;
-                p[r] = q < a.N ? weight(terms.score(a, p[r], q, k, cls[i], ck), top[i]) * inv[i] : 0.0f;
-                ds[r] = q < a.N ? p[r] * (ds[r] - delta[i]) : 0.0f;
+                const int i = first + r;
+                p[r] = q0 + i < a.N ? weight(p[r], top[i]) * inv[i] : 0.0f;
+                ds[r] = q0 + i < a.N ? p[r] * (ds[r] - delta[i]) : 0.0f;
             }
             accumulate<T, D>(dv, o_lds, 16 * t, round4<T>(p), col, g);
             accumulate<T, D>(dk, q_lds, 16 * t, round4<T>(ds), col, g);
@@ -382,14 +427,12 @@ __global__ void __launch_bounds__(kThreads) attn_grad_bias_kernel(const AttnArgs
         __syncthreads();
 #pragma unroll
         for (int t = 0; t < L::kRows / 16; ++t) {
-            const f32x4 s = product<T, D>(k_lds, 16 * t, qr, col, g);
+            const int i = 16 * t + 4 * g;
+            const f32x4 s = terms.of_query(a, product<T, D>(k_lds, 16 * t, qr, col, g), q, k0 + i, cq, cls + i);
             const f32x4 dp = product<T, D>(v_lds, 16 * t, go, col, g);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * t + 4 * g + r, k = k0 + i;
-                if (k < a.N)
-                    acc[t][r] += weight(terms.score(a, s[r], q, k, cq, cls[i]), top) * inv * (dp[r] - delta);
-            }
+            for (int r = 0; r < 4; ++r)
+                if (k0 + i + r < a.N) acc[t][r] += weight(s[r], top) * inv * (dp[r] - delta);
         }
     }
     if (q0 >= a.N) return;

@@ -19,21 +19,49 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kSegment = 2048;
 
-// Bits are copied, so one form per element size.  A workgroup writes 4 x 256
-// pairs of one head.  An index outside the table reads as 0.
+// Four neighbouring pairs at any address (a head's row begins at a multiple of
+// P): one wide access, which the memory takes at any alignment of an element.
 template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Four {
+    T v[4];
+};
+
+// Bits are copied, so one form per element size.  A workgroup writes `pairs`
+// pairs of one head, 4 a thread and step.  Where there is work for 256 of them
+// at 16384 pairs each, and the head's column of the table fits, the column waits
+// in LDS (kLds), since a gather of table rows touches one line a lane; smaller
+// calls gather, 1024 pairs to a workgroup.  An index outside the table reads as
+// 0.
+constexpr int64_t kManyPairs = 16384, kFewPairs = 1024;
+constexpr int kColumn = 16384;  // bytes of LDS for a column
+
+template <typename T, bool kLds>
 __global__ void __launch_bounds__(kThreads)
 bucket_bias_kernel(T* __restrict__ out, const T* __restrict__ table, const int32_t* __restrict__ index, int64_t P,
-                   int32_t L, int32_t H) {
+                   int32_t L, int32_t H, int32_t pairs) {
+    __shared__ T column[kLds ? kColumn / sizeof(T) : 1];
     const int h = static_cast<int>(blockIdx.y);
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * (4 * kThreads) + threadIdx.x;
+    if constexpr (kLds) {
+        for (int l = threadIdx.x; l < L; l += kThreads) column[l] = table[static_cast<int64_t>(l) * H + h];
+        __syncthreads();
+    }
+    const auto value = [&](int32_t l) {
+        if (static_cast<uint32_t>(l) >= static_cast<uint32_t>(L)) return T(0);
+        return kLds ? column[l] : table[static_cast<int64_t>(l) * H + h];
+    };
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * pairs;
+    const int64_t last = first + pairs < P ? first + pairs : P;
     T* to = out + h * P;
+    for (int64_t p = first + threadIdx.x * 4; p < last; p += kThreads * 4) {
+        if (p + 4 <= last) {
+            const Four<int32_t> l = *reinterpret_cast<const Four<int32_t>*>(index + p);
+            Four<T> v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t p = first + i * kThreads;
-        if (p >= P) break;
-        const int32_t l = index[p];
-        to[p] = static_cast<uint32_t>(l) < static_cast<uint32_t>(L) ? table[static_cast<int64_t>(l) * H + h] : T(0);
+            for (int e = 0; e < 4; ++e) v.v[e] = value(l.v[e]);
+            *reinterpret_cast<Four<T>*>(to + p) = v;
+        } else {
+            for (int64_t i = p; i < last; ++i) to[i] = value(index[i]);
+        }
     }
 }
 
@@ -42,8 +70,12 @@ template <typename T, typename To>
 __global__ void __launch_bounds__(kThreads)
 bucket_sum_kernel(To* __restrict__ out, const T* __restrict__ grad, const int32_t* __restrict__ order,
                   const int32_t* __restrict__ segments, int64_t P, int32_t H, uint32_t n) {
-    const uint32_t unit = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-    const int h = static_cast<int>(blockIdx.y), lane = threadIdx.x & 63;
+    // the workgroups of one head share an XCD, and its L2 the head's pairs
+    const uint32_t groups = (n + kThreads / 64 - 1) / (kThreads / 64);
+    uint32_t chunk;
+    if (!xcd_chunk(blockIdx.x, gridDim.x, groups * static_cast<uint32_t>(H), chunk)) return;
+    const uint32_t unit = chunk % groups * (kThreads / 64) + (threadIdx.x >> 6);
+    const int h = static_cast<int>(chunk / groups), lane = threadIdx.x & 63;
     if (unit >= n) return;
     const int64_t from = segments[2 * unit] < 0 ? 0 : segments[2 * unit];
     const int64_t to = segments[2 * unit + 1] < P ? segments[2 * unit + 1] : P;
@@ -86,9 +118,23 @@ int check(int32_t dtype, int64_t buckets, int64_t heads, int64_t pairs, const ch
 }
 
 template <typename T>
+void forward(void* out, const void* table, const int32_t* index, int64_t L, int64_t H, int64_t P, hipStream_t s) {
+    const bool lds = P * H >= 256 * kManyPairs && L <= static_cast<int64_t>(kColumn / sizeof(T));
+    const int64_t pairs = lds ? kManyPairs : kFewPairs;
+    const dim3 grid(static_cast<uint32_t>((P + pairs - 1) / pairs), static_cast<uint32_t>(H));
+    T* o = static_cast<T*>(out);
+    const T* t = static_cast<const T*>(table);
+    const int32_t l = static_cast<int32_t>(L), h = static_cast<int32_t>(H);
+    if (lds)
+        bucket_bias_kernel<T, true><<<grid, kThreads, 0, s>>>(o, t, index, P, l, h, static_cast<int32_t>(pairs));
+    else
+        bucket_bias_kernel<T, false><<<grid, kThreads, 0, s>>>(o, t, index, P, l, h, static_cast<int32_t>(pairs));
+}
+
+template <typename T>
 int backward(void* grad_table, const void* grad, int64_t L, int64_t H, int64_t P, const int32_t* order,
              const int32_t* segments, int64_t n, const int32_t* firsts, float* partial, hipStream_t s) {
-    const dim3 grid(static_cast<uint32_t>((n + 3) / 4), static_cast<uint32_t>(H));
+    const uint32_t grid = xcd_launch_count(static_cast<uint32_t>((n + 3) / 4 * H));
     const T* g = static_cast<const T*>(grad);
     if (firsts == nullptr) {  // one segment a bucket
         bucket_sum_kernel<T, T><<<grid, kThreads, 0, s>>>(static_cast<T*>(grad_table), g, order, segments, P,
@@ -116,18 +162,11 @@ extern "C" int crumpet_bucket_bias(void* out, const void* table, int32_t dtype, 
     if (st != CRUMPET_OK || heads == 0 || pairs == 0) return st;
     if (out == nullptr || table == nullptr || index == nullptr)
         return fail(CRUMPET_ERR_INVALID_ARGUMENT, "bucket_bias: null tensor");
-    const dim3 grid(static_cast<uint32_t>((pairs + 4 * kThreads - 1) / (4 * kThreads)), static_cast<uint32_t>(heads));
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == CRUMPET_DTYPE_F32)
-        bucket_bias_kernel<uint32_t><<<grid, kThreads, 0, s>>>(static_cast<uint32_t*>(out),
-                                                               static_cast<const uint32_t*>(table), index, pairs,
-                                                               static_cast<int32_t>(buckets),
-                                                               static_cast<int32_t>(heads));
+        forward<uint32_t>(out, table, index, buckets, heads, pairs, s);
     else
-        bucket_bias_kernel<uint16_t><<<grid, kThreads, 0, s>>>(static_cast<uint16_t*>(out),
-                                                               static_cast<const uint16_t*>(table), index, pairs,
-                                                               static_cast<int32_t>(buckets),
-                                                               static_cast<int32_t>(heads));
+        forward<uint16_t>(out, table, index, buckets, heads, pairs, s);
     return check_launch("bucket_bias");
 }
 
@@ -145,7 +184,7 @@ extern "C" int crumpet_bucket_bias_backward(void* grad_table, const void* grad, 
     if (firsts != nullptr && workspace == nullptr)
         return fail(CRUMPET_ERR_INVALID_ARGUMENT, "%s: null workspace", what);
     if (!launch_takes(static_cast<uint64_t>(buckets) * heads / 4 + 1, kThreads) ||
-        !launch_takes(static_cast<uint64_t>(segment_count) / 4 + 1, kThreads))
+        !launch_takes((static_cast<uint64_t>(segment_count) / 4 + 1) * heads + kNumXcd, kThreads))
         return fail(CRUMPET_ERR_UNSUPPORTED, "%s: too many buckets or segments for one launch", what);
     hipStream_t s = static_cast<hipStream_t>(stream);
     float* partial = static_cast<float*>(workspace);

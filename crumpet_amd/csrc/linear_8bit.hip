@@ -134,71 +134,98 @@ __global__ void __launch_bounds__(kThreads) linear_8bit_rows_kernel(const RowsAr
         row[r] = row0 + 16 * r;
         xr[r] = static_cast<const T*>(a.x) + (row[r] < a.rows ? row[r] : a.rows - 1) * a.K;
     }
+    // Row m of tile n is feature 4 NT (m / 4) + 4 n + m % 4 of the block, so that
+    // a lane ends with 4 NT neighbouring features of its row.
     const T* wr[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int f = n0 + 16 * n + col;
+        const int f = n0 + 4 * NT * (col >> 2) + 4 * n + (col & 3);
         wr[n] = static_cast<const T*>(a.w) + static_cast<int64_t>(f < a.n_out ? f : a.n_out - 1) * a.K;
     }
-    f32x4 acc[NT][2] = {};
-    for (int k0 = 0; k0 < a.K; k0 += kGroup) {
+    // K is a multiple of 16: the last step may be half a group
+    X8 xv[2], wv[NT];
+    const auto fetch = [&](int k0) {
         const int k = k0 + 8 * g;
-        const bool in = k < a.K;  // K is a multiple of 16: a last half step
-        X8 xv[2];
+        const bool in = k < a.K;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             xv[r] = X8{};
             if (in) xv[r] = *reinterpret_cast<const X8*>(xr[r] + k);
         }
-        X8 wv[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             wv[n] = X8{};
             if (in) wv[n] = *reinterpret_cast<const X8*>(wr[n] + k);
         }
+    };
+    f32x4 acc[NT][2] = {};
+    fetch(0);
+    for (int k0 = 0; k0 < a.K; k0 += kGroup) {
+        X8 x[2] = {xv[0], xv[1]}, w[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) w[n] = wv[n];
+        if (k0 + kGroup < a.K) fetch(k0 + kGroup);
         if constexpr (kForward) {
+            const int k = k0 + 8 * g;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 if (keep) {
                     int e;
-                    const i8x8 codes = quantise<T>(xv[r], e);
+                    const i8x8 codes = quantise<T>(x[r], e);
                     if (row[r] < a.rows) {
-                        if (in) *reinterpret_cast<i8x8*>(a.codes + row[r] * a.K + k) = codes;
+                        if (k < a.K) *reinterpret_cast<i8x8*>(a.codes + row[r] * a.K + k) = codes;
                         if (g == 0) a.exps[row[r] * groups + k0 / kGroup] = static_cast<int8_t>(e);
                     }
                 }
                 if constexpr (kGelu) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) xv[r][i] = static_cast<T>(act<true>(static_cast<float>(xv[r][i])));
+                    for (int i = 0; i < 8; ++i) x[r][i] = static_cast<T>(act<true>(static_cast<float>(x[r][i])));
                 }
             }
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) acc[n][r] = Mma<T>::mma32(wv[n], xv[r], acc[n][r]);
+            for (int r = 0; r < 2; ++r) acc[n][r] = Mma<T>::mma32(w[n], x[r], acc[n][r]);
         }
     }
     const int out_groups = (a.n_out + kGroup - 1) / kGroup;
+    const int f0 = n0 + 4 * NT * g;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int f = n0 + 16 * n + 4 * g;
-        if (f >= a.n_out) continue;
-        f32x4 bias = {};
-        if (kForward && a.b != nullptr) bias = wide4<T>(load4<T>(static_cast<const T*>(a.b) + f));
+    for (int r = 0; r < 2; ++r) {
+        if (row[r] >= a.rows) continue;
+        T* to = static_cast<T*>(a.y) + row[r] * a.n_out + f0;
+        // two tiles are 8 neighbouring features: 16 bytes, aligned where NT is even
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            if (row[r] >= a.rows) continue;
-            f32x4 v = acc[n][r];
-            if constexpr (kForward) {
-                v += bias;
-            } else if constexpr (kGelu) {
-                const i8x4 c = *reinterpret_cast<const i8x4*>(a.codes + row[r] * a.n_out + f);
-                const float step = power_of_two(a.exps[row[r] * out_groups + f / kGroup]);
+        for (int n = 0; n < NT; n += NT % 2 == 0 ? 2 : 1) {
+            constexpr int kEach = NT % 2 == 0 ? 2 : 1;
+            f32x4 v[kEach];
+            bool in[kEach];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] *= act_grad<true>(static_cast<float>(c[i]) * step);
+            for (int u = 0; u < kEach; ++u) {
+                const int f = f0 + 4 * (n + u);
+                in[u] = f < a.n_out;
+                v[u] = acc[n + u][r];
+                if (!in[u]) continue;
+                if constexpr (kForward) {
+                    if (a.b != nullptr) v[u] += wide4<T>(load4<T>(static_cast<const T*>(a.b) + f));
+                } else if constexpr (kGelu) {
+                    const i8x4 c = *reinterpret_cast<const i8x4*>(a.codes + row[r] * a.n_out + f);
+                    const float step = power_of_two(a.exps[row[r] * out_groups + f / kGroup]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[u][i] *= act_grad<true>(static_cast<float>(c[i]) * step);
+                }
             }
-            *reinterpret_cast<typename Mma<T>::x4*>(static_cast<T*>(a.y) + row[r] * a.n_out + f) = round4<T>(v);
+            if constexpr (kEach == 2) {
+                if (in[1]) {
+                    const typename Mma<T>::x4 lo = round4<T>(v[0]), hi = round4<T>(v[1]);
+                    *reinterpret_cast<X8*>(to + 4 * n) = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                    continue;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kEach; ++u)
+                if (in[u]) *reinterpret_cast<typename Mma<T>::x4*>(to + 4 * (n + u)) = round4<T>(v[u]);
         }
     }
 }
@@ -253,30 +280,42 @@ __global__ void __launch_bounds__(kThreads) linear_8bit_weight_kernel(const Weig
     X8 ones;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ones[i] = static_cast<T>(1.0f);
+    // the rows of the next step, on their way while this one's are multiplied
+    X8 dy_next[2];
+    i8x16 codes_next[2];
+    int e_next[2];
+    const auto fetch = [&](int64_t r0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int p = threadIdx.x + i * kThreads, r = p >> 3, c = p & 7;
+            dy_next[i] = X8{};
+            codes_next[i] = i8x16{};
+            e_next[i] = 0;
+            if (r0 + r >= end) continue;
+            if (n0 + c * 8 < a.n_out)
+                dy_next[i] = *reinterpret_cast<const X8*>(static_cast<const T*>(a.dy) + (r0 + r) * a.n_out + n0 + c * 8);
+            if (k0 + c * 16 < a.K) {
+                codes_next[i] = *reinterpret_cast<const i8x16*>(a.codes + (r0 + r) * a.K + k0 + c * 16);
+                e_next[i] = a.exps[(r0 + r) * groups + (k0 + c * 16) / kGroup];
+            }
+        }
+    };
+    if (begin < end) fetch(begin);
     for (int64_t r0 = begin; r0 < end; r0 += kRows) {
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int p = threadIdx.x + i * kThreads, r = p >> 3, c = (p & 7) * 8;
-            X8 v = {};
-            if (r0 + r < end && n0 + c < a.n_out)
-                v = *reinterpret_cast<const X8*>(static_cast<const T*>(a.dy) + (r0 + r) * a.n_out + n0 + c);
-            *reinterpret_cast<X8*>(dy_lds + r * kLdN + c) = v;
-        }
+            const int p = threadIdx.x + i * kThreads, r = p >> 3, c = p & 7;
+            *reinterpret_cast<X8*>(dy_lds + r * kLdN + c * 8) = dy_next[i];
+            X8 v[2];
+            const float step = power_of_two(e_next[i]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int p = threadIdx.x + i * kThreads, r = p >> 3, c = (p & 7) * 16;
-            X8 v[2] = {};
-            if (r0 + r < end && k0 + c < a.K) {
-                const i8x16 codes = *reinterpret_cast<const i8x16*>(a.codes + (r0 + r) * a.K + k0 + c);
-                const float step = power_of_two(a.exps[(r0 + r) * groups + (k0 + c) / kGroup]);
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    v[e >> 3][e & 7] = static_cast<T>(act<kGelu>(static_cast<float>(codes[e]) * step));
-            }
-            *reinterpret_cast<X8*>(x_lds + r * kLdK + c) = v[0];
-            *reinterpret_cast<X8*>(x_lds + r * kLdK + c + 8) = v[1];
+            for (int e = 0; e < 16; ++e)
+                v[e >> 3][e & 7] = static_cast<T>(act<kGelu>(static_cast<float>(codes_next[i][e]) * step));
+            *reinterpret_cast<X8*>(x_lds + r * kLdK + c * 16) = v[0];
+            *reinterpret_cast<X8*>(x_lds + r * kLdK + c * 16 + 8) = v[1];
         }
+        if (r0 + kRows < end) fetch(r0 + kRows);
         __syncthreads();
 #pragma unroll
         for (int s = 0; s < kRows; s += 32) {
@@ -319,15 +358,26 @@ __global__ void __launch_bounds__(kThreads) linear_8bit_weight_kernel(const Weig
     }
 }
 
-// Chunks added in order; the first `weights` sums go to dw, the rest to db.
+// Sums of the chunks: 32 numbers by 8 groups of chunks per workgroup, each group
+// and then the groups in order; the first `weights` sums go to dw, the rest to
+// db.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) linear_8bit_join_kernel(T* dw, T* db, const float* __restrict__ partial,
                                                                    int64_t weights, int64_t all, int64_t chunks) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-    if (i >= all) return;
+    __shared__ float lds[8][33];
+    const int x = threadIdx.x & 31, part = threadIdx.x >> 5;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 32 + x;
     float v = 0.0f;
+    if (i < all) {
 #pragma unroll 8
-    for (int64_t c = 0; c < chunks; ++c) v += partial[c * all + i];
+        for (int64_t c = part; c < chunks; c += 8) v += partial[c * all + i];
+    }
+    lds[part][x] = v;
+    __syncthreads();
+    if (part != 0 || i >= all) return;
+    v = 0.0f;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) v += lds[p][x];
     if (i < weights) {
         if (dw != nullptr) dw[i] = static_cast<T>(v);
     } else if (db != nullptr) {
@@ -418,7 +468,7 @@ int backward(void* dx, void* dw, void* db, const void* dy, const int8_t* codes, 
     else
         linear_8bit_weight_kernel<T, false><<<grid, kThreads, 0, s>>>(a);
     const int64_t all = n_out * K + n_out;
-    linear_8bit_join_kernel<T><<<static_cast<uint32_t>((all + kThreads - 1) / kThreads), kThreads, 0, s>>>(
+    linear_8bit_join_kernel<T><<<static_cast<uint32_t>((all + 31) / 32), kThreads, 0, s>>>(
         static_cast<T*>(dw), static_cast<T*>(db), a.partial, n_out * K, all, p.chunks);
     return check_launch("linear_8bit_backward");
 }

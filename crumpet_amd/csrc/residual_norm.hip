@@ -90,6 +90,8 @@ struct Lane {
             in[i] = at[i] < C;  // C is a multiple of E
         }
     }
+    // dflt where there is no row; 0 past it, so that a product with it ends
+    // what sums over the row must not see
     template <typename T>
     __device__ __forceinline__ void load(const T* row, float* v, float dflt = 0.0f) const {
 #pragma unroll
@@ -98,7 +100,7 @@ struct Lane {
                 load_row<T, E>(row + at[i], v + i * E);
             } else {
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[i * E + e] = dflt;
+                for (int e = 0; e < E; ++e) v[i * E + e] = in[i] ? dflt : 0.0f;
             }
         }
     }
@@ -133,7 +135,8 @@ struct Lane {
         for (int i = 0; i < NV * E; ++i) v[i] *= r;
         return r;
     }
-    // g (gradient of the normed values n) -> gradient of the values; 0 past the row
+    // g (gradient of the normed values n, 0 past the row) -> gradient of the
+    // values, anything past the row
     __device__ __forceinline__ void normalise_grad(float* g, const float* n, float r, int C, bool rms, float* lds) const {
         const float per = 1.0f / static_cast<float>(C);
         float a = 0.0f, c = 0.0f;
@@ -145,10 +148,7 @@ struct Lane {
         a = rms ? 0.0f : row_sum<G>(a, lds) * per;
         c = row_sum<G>(c, lds) * per;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-#pragma unroll
-            for (int e = i * E; e < (i + 1) * E; ++e) g[e] = in[i] ? r * (g[e] - a - n[e] * c) : 0.0f;
-        }
+        for (int i = 0; i < NV * E; ++i) g[i] = r * (g[i] - a - n[i] * c);
     }
 };
 
@@ -190,56 +190,74 @@ __global__ void __launch_bounds__(kThreads) residual_norm_kernel(const NormArgs 
     }
 }
 
-template <typename Tx, typename Ty, int E, int NV, int G>
+// Parameters are loaded where they are used, again if need be: they come from
+// the cache, and rows, their norms and the sums fill the registers.
+template <typename Tx, typename Ty, int E, int NV, int G, bool kPost>
 __global__ void __launch_bounds__(kThreads) residual_norm_grad_kernel(const NormArgs a) {
-    constexpr int kRows = kThreads / G, kN = NV * E, kCols = G * kN;
+    constexpr int kRows = kThreads / G, kN = NV * E, kCols = G * kN, kMine = kPost ? kSums : 3;
     __shared__ float lds[kRows > 1 ? kThreads * kN : 4];
     const Lane<E, NV, G> lane(a.C);
     const uint32_t sample = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
     const float k = a.scale != nullptr ? a.scale[sample] : 1.0f;
     const float* gate = a.gate != nullptr ? a.gate + static_cast<int64_t>(sample) * a.gate_stride : nullptr;
-    float sums[kSums][kN] = {};
+    float sums[kMine][kN] = {};
     const uint32_t step = a.chunks * kRows;
     for (uint32_t t = chunk * kRows + threadIdx.x / G; t < a.T; t += step) {
         const int64_t row = (static_cast<int64_t>(sample) * a.T + t) * a.C;
-        float n[kN], y[kN], gx[kN], kg[kN], p[kN], yr = 0.0f;
+        float n[kN], y[kN], gx[kN], other[kN], yr = 0.0f;
         lane.load(static_cast<const Tx*>(a.x) + row, n);
         lane.load(static_cast<const Ty*>(a.y) + row, y);
         lane.load(a.gout != nullptr ? static_cast<const Ty*>(a.gout) + row : nullptr, gx);
-        lane.load(gate, kg, 1.0f);
-        if (a.post) yr = lane.normalise(y, a.C, a.rms, a.post_eps, lds);
-        float u[kN];
-        if (a.post) {
-            lane.load(a.pw, p, 1.0f);
-            lane.load(a.pb, u);
+        lane.load(a.gsum != nullptr ? static_cast<const Tx*>(a.gsum) + row : nullptr, other);
+        if constexpr (kPost) yr = lane.normalise(y, a.C, a.rms, a.post_eps, lds);
+        // y' = y p + b, made again where it is needed again
+        const auto branch = [&](float* u) {
+            if constexpr (kPost) {
+                float p[kN];
+                lane.load(a.pw, p, 1.0f);
+                lane.load(a.pb, u);
 #pragma unroll
-            for (int i = 0; i < kN; ++i) u[i] = __builtin_fmaf(y[i], p[i], u[i]);
-        } else {
+                for (int i = 0; i < kN; ++i) u[i] = __builtin_fmaf(y[i], p[i], u[i]);
+            } else {
 #pragma unroll
-            for (int i = 0; i < kN; ++i) u[i] = y[i];
+                for (int i = 0; i < kN; ++i) u[i] = y[i];
+            }
+        };
+        {
+            float kg[kN], u[kN];
+            lane.load(gate, kg, 1.0f);
+            branch(u);
+#pragma unroll
+            for (int i = 0; i < kN; ++i) n[i] = __builtin_fmaf(k * kg[i], u[i], n[i]);
         }
-#pragma unroll
-        for (int i = 0; i < kN; ++i) n[i] = __builtin_fmaf(k * kg[i], u[i], n[i]);
         const float r = lane.normalise(n, a.C, a.rms, a.eps, lds);
-        float w[kN];
-        lane.load(a.w, w, 1.0f);
+        {
+            float w[kN];
+            lane.load(a.w, w, 1.0f);
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            sums[0][i] = __builtin_fmaf(gx[i], n[i], sums[0][i]);
-            sums[1][i] += gx[i];
-            gx[i] *= w[i];
+            for (int i = 0; i < kN; ++i) {
+                sums[0][i] = __builtin_fmaf(gx[i], n[i], sums[0][i]);
+                sums[1][i] += gx[i];
+                gx[i] *= w[i];
+            }
         }
         lane.normalise_grad(gx, n, r, a.C, a.rms, lds);
-        lane.load(a.gsum != nullptr ? static_cast<const Tx*>(a.gsum) + row : nullptr, n);
 #pragma unroll
-        for (int i = 0; i < kN; ++i) gx[i] += n[i];
+        for (int i = 0; i < kN; ++i) gx[i] += other[i];
         lane.store(static_cast<Tx*>(a.gx) + row, gx);
+        {
+            float kg[kN], u[kN];
+            lane.load(gate, kg, 1.0f);
+            branch(u);
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            sums[2][i] = __builtin_fmaf(gx[i] * k, u[i], sums[2][i]);
-            gx[i] *= k * kg[i];
+            for (int i = 0; i < kN; ++i) {
+                sums[2][i] = __builtin_fmaf(gx[i] * k, u[i], sums[2][i]);
+                gx[i] *= k * kg[i];
+            }
         }
-        if (a.post) {
+        if constexpr (kPost) {
+            float p[kN];
+            lane.load(a.pw, p, 1.0f);
 #pragma unroll
             for (int i = 0; i < kN; ++i) {
                 sums[3][i] = __builtin_fmaf(gx[i], y[i], sums[3][i]);
@@ -253,9 +271,9 @@ __global__ void __launch_bounds__(kThreads) residual_norm_grad_kernel(const Norm
     if (a.partial == nullptr) return;
     float* to = a.partial + static_cast<int64_t>(blockIdx.x) * kSums * a.C;
 #pragma unroll
-    for (int s = 0; s < kSums; ++s) {
+    for (int s = 0; s < kMine; ++s) {
         // uniform over the launch: the sums that somebody reads
-        if ((s == 2 && a.gate == nullptr) || (s >= 3 && !a.post)) continue;
+        if (s == 2 && a.gate == nullptr) continue;
         if constexpr (kRows > 1) {
             __syncthreads();
 #pragma unroll
@@ -276,7 +294,8 @@ __global__ void __launch_bounds__(kThreads) residual_norm_grad_kernel(const Norm
     }
 }
 
-// Sums of the partial rows: 16 columns by 16 groups of rows per workgroup.
+// Sums of the partial rows: 16 columns by 64 groups of rows per workgroup.
+constexpr int kParts = 64;
 struct SumArgs {
     const float* partial;
     float* out[kSums];     // null where nobody asked
@@ -285,8 +304,8 @@ struct SumArgs {
     int32_t C;
 };
 
-__global__ void __launch_bounds__(kThreads) residual_norm_sums_kernel(const SumArgs a) {
-    __shared__ float lds[16][17];
+__global__ void __launch_bounds__(kParts * 16) residual_norm_sums_kernel(const SumArgs a) {
+    __shared__ float lds[kParts][17];
     const int which = static_cast<int>(blockIdx.y);
     if (a.out[which] == nullptr) return;
     const uint32_t samples = a.per_sample[which] ? a.S : 1u;
@@ -297,20 +316,23 @@ __global__ void __launch_bounds__(kThreads) residual_norm_sums_kernel(const SumA
     float v = 0.0f;
     if (c < a.C) {
 #pragma unroll 4
-        for (uint32_t r = part; r < rows; r += 16) v += from[static_cast<int64_t>(r) * kSums * a.C];
+        for (uint32_t r = part; r < rows; r += kParts) v += from[static_cast<int64_t>(r) * kSums * a.C];
     }
     lds[part][threadIdx.x & 15] = v;
     __syncthreads();
     if (part != 0 || c >= a.C) return;
     v = 0.0f;
-    for (int i = 0; i < 16; ++i) v += lds[i][threadIdx.x];
+#pragma unroll 8
+    for (int i = 0; i < kParts; ++i) v += lds[i][threadIdx.x];
     a.out[which][static_cast<int64_t>(blockIdx.z) * a.C + c] = v;
 }
 
 template <typename Tx, typename Ty, int E, int NV, int G>
 void launch(const NormArgs& a, bool grad, hipStream_t s) {
-    if (grad)
-        residual_norm_grad_kernel<Tx, Ty, E, NV, G><<<a.S * a.chunks, kThreads, 0, s>>>(a);
+    if (grad && a.post)
+        residual_norm_grad_kernel<Tx, Ty, E, NV, G, true><<<a.S * a.chunks, kThreads, 0, s>>>(a);
+    else if (grad)
+        residual_norm_grad_kernel<Tx, Ty, E, NV, G, false><<<a.S * a.chunks, kThreads, 0, s>>>(a);
     else
         residual_norm_kernel<Tx, Ty, E, NV, G><<<a.S * a.chunks, kThreads, 0, s>>>(a);
 }
@@ -460,6 +482,6 @@ extern "C" int crumpet_residual_norm_backward(
     f.per_sample[2] = gate_per_sample;
     f.S = a.S, f.chunks = a.chunks, f.C = a.C;
     const uint32_t deep = grad_gate != nullptr && gate_per_sample ? a.S : 1u;
-    residual_norm_sums_kernel<<<dim3((a.C + 15) / 16, kSums, deep), kThreads, 0, s>>>(f);
+    residual_norm_sums_kernel<<<dim3((a.C + 15) / 16, kSums, deep), kParts * 16, 0, s>>>(f);
     return check_launch(what);
 }
