@@ -31,9 +31,6 @@ constexpr int kThreads = 256;
 constexpr int kGroup = 32;
 constexpr int kNaN = -128;  // exponent byte of a group that is not finite
 
-typedef int8_t i8x4 __attribute__((ext_vector_type(4)));
-typedef int8_t i8x8 __attribute__((ext_vector_type(8)));
-typedef int8_t i8x16 __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ float power_of_two(int e) {
     return e == kNaN ? __builtin_nanf("") : __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
@@ -72,35 +69,60 @@ __device__ __forceinline__ float act_grad(float x) {
     return 1.0f;
 }
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
 // Codes of 8 of a group's 32 values (the other lanes of the row hold the
-// rest), and the group's exponent.  Magnitudes compare as their bits, NaN
+// rest), and the group's exponent.  Magnitudes compare as their 16 bits, NaN
 // above everything.
 template <typename T>
-__device__ __forceinline__ i8x8 quantise(typename Mma<T>::x8 v, int& e) {
-    uint32_t top = 0;
+__device__ __forceinline__ u32x2 quantise(typename Mma<T>::x8 v, int& e) {
+    const u32x4 raw = __builtin_bit_cast(u32x4, v);
+    uint32_t top = 0;  // in the upper half
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t bits = __float_as_uint(static_cast<float>(v[i])) & 0x7fffffffu;
-        top = top > bits ? top : bits;
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t hi = raw[i] & 0x7fff0000u, lo = (raw[i] & 0x7fffu) << 16, more = hi > lo ? hi : lo;
+        top = top > more ? top : more;
     }
 #pragma unroll
     for (int m = 16; m <= 32; m <<= 1) {
         const uint32_t other = __shfl_xor(top, m);
         top = top > other ? top : other;
     }
-    // top = 1.f 2^k; 127 = 1.984375 2^6
-    const int k = static_cast<int>(top >> 23) - 127;
-    e = k - ((top & 0x7fffffu) > 0x7e0000u ? 5 : 6);
+    const uint32_t bits =
+        __float_as_uint(static_cast<float>(__builtin_bit_cast(T, static_cast<unsigned short>(top >> 16))));
+    // the largest magnitude is 1.f 2^k; 127 = 1.984375 2^6
+    const int k = static_cast<int>(bits >> 23) - 127;
+    e = k - ((bits & 0x7fffffu) > 0x7e0000u ? 5 : 6);
     e = e < -126 ? -126 : e;
-    i8x8 codes = {};
-    if (top >= 0x7f800000u) {
+    if (bits >= 0x7f800000u) {
         e = kNaN;
-        return codes;
+        return u32x2{};
     }
     const float up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+    // x 2^-e + 1.5 2^23 is the rounded code in the low bits of the mantissa
+    uint32_t c[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) codes[i] = static_cast<int8_t>(__builtin_rintf(static_cast<float>(v[i]) * up));
+    for (int i = 0; i < 8; ++i)
+        c[i] = __float_as_uint(__builtin_fmaf(static_cast<float>(v[i]), up, 12582912.0f));
+    u32x2 codes;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t lo = __builtin_amdgcn_perm(c[4 * i + 1], c[4 * i], 0x0c0c0400u);
+        const uint32_t hi = __builtin_amdgcn_perm(c[4 * i + 3], c[4 * i + 2], 0x0c0c0400u);
+        codes[i] = hi << 16 | lo;
+    }
     return codes;
+}
+
+// Four codes times the group's step: (code + 128) step - 128 step, exact, with
+// one conversion of an unsigned byte each.
+__device__ __forceinline__ f32x4 values_of(uint32_t codes, float step) {
+    const uint32_t u = codes ^ 0x80808080u;
+    const float less = -128.0f * step;
+    f32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(static_cast<float>((u >> (8 * i)) & 0xffu), step, less);
+    return v;
 }
 
 struct RowsArgs {
@@ -171,9 +193,9 @@ __global__ void __launch_bounds__(kThreads) linear_8bit_rows_kernel(const RowsAr
             for (int r = 0; r < 2; ++r) {
                 if (keep) {
                     int e;
-                    const i8x8 codes = quantise<T>(x[r], e);
+                    const u32x2 codes = quantise<T>(x[r], e);
                     if (row[r] < a.rows) {
-                        if (k < a.K) *reinterpret_cast<i8x8*>(a.codes + row[r] * a.K + k) = codes;
+                        if (k < a.K) *reinterpret_cast<u32x2*>(a.codes + row[r] * a.K + k) = codes;
                         if (g == 0) a.exps[row[r] * groups + k0 / kGroup] = static_cast<int8_t>(e);
                     }
                 }
@@ -210,10 +232,10 @@ __global__ void __launch_bounds__(kThreads) linear_8bit_rows_kernel(const RowsAr
                 if constexpr (kForward) {
                     if (a.b != nullptr) v[u] += wide4<T>(load4<T>(static_cast<const T*>(a.b) + f));
                 } else if constexpr (kGelu) {
-                    const i8x4 c = *reinterpret_cast<const i8x4*>(a.codes + row[r] * a.n_out + f);
-                    const float step = power_of_two(a.exps[row[r] * out_groups + f / kGroup]);
+                    const f32x4 x = values_of(*reinterpret_cast<const uint32_t*>(a.codes + row[r] * a.n_out + f),
+                                              power_of_two(a.exps[row[r] * out_groups + f / kGroup]));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) v[u][i] *= act_grad<true>(static_cast<float>(c[i]) * step);
+                    for (int i = 0; i < 4; ++i) v[u][i] *= act_grad<true>(x[i]);
                 }
             }
             if constexpr (kEach == 2) {
@@ -282,20 +304,20 @@ __global__ void __launch_bounds__(kThreads) linear_8bit_weight_kernel(const Weig
     for (int i = 0; i < 8; ++i) ones[i] = static_cast<T>(1.0f);
     // the rows of the next step, on their way while this one's are multiplied
     X8 dy_next[2];
-    i8x16 codes_next[2];
+    u32x4 codes_next[2];
     int e_next[2];
     const auto fetch = [&](int64_t r0) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int p = threadIdx.x + i * kThreads, r = p >> 3, c = p & 7;
             dy_next[i] = X8{};
-            codes_next[i] = i8x16{};
+            codes_next[i] = u32x4{};
             e_next[i] = 0;
             if (r0 + r >= end) continue;
             if (n0 + c * 8 < a.n_out)
                 dy_next[i] = *reinterpret_cast<const X8*>(static_cast<const T*>(a.dy) + (r0 + r) * a.n_out + n0 + c * 8);
             if (k0 + c * 16 < a.K) {
-                codes_next[i] = *reinterpret_cast<const i8x16*>(a.codes + (r0 + r) * a.K + k0 + c * 16);
+                codes_next[i] = *reinterpret_cast<const u32x4*>(a.codes + (r0 + r) * a.K + k0 + c * 16);
                 e_next[i] = a.exps[(r0 + r) * groups + (k0 + c * 16) / kGroup];
             }
         }
@@ -310,8 +332,11 @@ __global__ void __launch_bounds__(kThreads) linear_8bit_weight_kernel(const Weig
             X8 v[2];
             const float step = power_of_two(e_next[i]);
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                v[e >> 3][e & 7] = static_cast<T>(act<kGelu>(static_cast<float>(codes_next[i][e]) * step));
+            for (int w = 0; w < 4; ++w) {
+                const f32x4 x = values_of(codes_next[i][w], step);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[w >> 1][4 * (w & 1) + e] = static_cast<T>(act<kGelu>(x[e]));
+            }
             *reinterpret_cast<X8*>(x_lds + r * kLdK + c * 16) = v[0];
             *reinterpret_cast<X8*>(x_lds + r * kLdK + c * 16 + 8) = v[1];
         }
