@@ -13,9 +13,9 @@
 // Scores, softmax, delta and dS are fp32; P and dS are rounded to the input
 // type only as operands of the products whose results are rounded to it too.
 // dbias sums the unrounded dS, and delta enters it in fp32: for training the
-// product P v takes P as its rounded value and the rest, and out is kept the
-// same way (with P rounded once dbias is off by 2e-5 in fp16 and 2e-4 in bf16,
-// against 2e-7).
+// product P v takes P as its rounded value and the rest, and out is kept with
+// its rest (round_and_rest).  dbias is then off by 3e-7 in fp16 and 3 to 9e-7
+// in bf16; with P rounded once it is 2e-5 and 2e-4.
 #pragma once
 
 #include <algorithm>
@@ -248,13 +248,12 @@ __global__ void __launch_bounds__(kThreads) attn_forward_kernel(const AttnArgs a
     const int64_t at = (static_cast<int64_t>(b) * a.N + q) * a.H + h;
 #pragma unroll
     for (int d = 0; d < L::kSlices; ++d) {
-        const f32x4 o = acc[d] * inv;
-        const typename Mma<T>::x4 hi = round4<T>(o);
+        typename Mma<T>::x4 hi, lo;
+        round_and_rest<T>(acc[d] * inv, hi, lo);
         *reinterpret_cast<typename Mma<T>::x4*>(static_cast<T*>(a.out) + at * D + 16 * d + 4 * g) = hi;
         if constexpr (sizeof(T) == 2) {
             if (a.out_lo != nullptr)
-                *reinterpret_cast<typename Mma<T>::x4*>(static_cast<T*>(a.out_lo) + at * D + 16 * d + 4 * g) =
-                    round4<T>(o - wide4<T>(hi));
+                *reinterpret_cast<typename Mma<T>::x4*>(static_cast<T*>(a.out_lo) + at * D + 16 * d + 4 * g) = lo;
         }
     }
     if (g == 0 && a.row_max != nullptr) {
@@ -276,8 +275,11 @@ __device__ __forceinline__ float row_delta(const AttnArgs& a, int64_t at, const 
     for (int s = 0; s < D / 16; ++s) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float x = static_cast<float>(o.v[s][e]);
-            if constexpr (sizeof(T) == 2) x += static_cast<float>(lo.v[s][e]);
+            float x;
+            if constexpr (sizeof(T) == 2)
+                x = with_rest<T>(o.v[s][e], lo.v[s][e]);
+            else
+                x = o.v[s][e];
             sum = __builtin_fmaf(x, static_cast<float>(go.v[s][e]), sum);
         }
     }

@@ -470,10 +470,10 @@ attn_forward_tuned_kernel(const AttnArgs a, const Order o, const Walk w) {
 #pragma unroll
         for (int d = 0; d < kOut; ++d) {
             const uint32_t lane_at = static_cast<uint32_t>(q) * (a.H * D) + 16 * d + 4 * g;
-            const f32x4 out = acc[d] * inv;
-            const X4 hi = round4<T>(out);
+            X4 hi, lo;
+            round_and_rest<T>(acc[d] * inv, hi, lo);
             *reinterpret_cast<X4*>(to + lane_at) = hi;
-            if (a.out_lo != nullptr) *reinterpret_cast<X4*>(to_lo + lane_at) = round4<T>(out - wide4<T>(hi));
+            if (a.out_lo != nullptr) *reinterpret_cast<X4*>(to_lo + lane_at) = lo;
         }
         if (g == 0 && a.row_max != nullptr) {
             const int64_t row = (static_cast<int64_t>(b) * a.H + h) * a.N;
@@ -665,7 +665,7 @@ attn_grad_q_tuned_kernel(const AttnArgs a, const Order o, const Walk w) {
             }
             float delta = 0.0f;
 #pragma unroll
-            for (int e = 0; e < D / 4; ++e) delta = __builtin_fmaf(out.dim(e) + rest.dim(e), go.dim(e), delta);
+            for (int e = 0; e < D / 4; ++e) delta = __builtin_fmaf(with_rest<T>(out.v[e], rest.v[e]), go.dim(e), delta);
             delta = sum_groups(delta);
             if (me.leads && g == 0 && me.row0 < a.N)
                 (a.delta + (static_cast<int64_t>(here.b) * a.H + h) * a.N)[static_cast<uint32_t>(q)] = delta;

@@ -10,6 +10,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "crumpet_common.h"
 #include "crumpet_hip.h"
 
@@ -77,6 +79,45 @@ __device__ __forceinline__ f32x4 wide4(typename Mma<T>::x4 v) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = static_cast<float>(v[e]);
     return o;
+}
+
+// An fp32 number kept as its rounding to T and a second value of 16 bits.  fp16:
+// the rounding of what is left, 2^-22 of the number.  bf16, whose rest would be
+// short at 2^-17: the bits below it, fp32's own, as a whole number in
+// [-2^15, 2^15) of fp32 steps (a tie that rounds down is one step less).
+//
+// v passes through the asm so that both see one number: a product formed anew
+// inside a fused conversion to fp16 rounds a near tie the other way, and lo
+// would not belong to hi.
+template <typename T>
+__device__ __forceinline__ void round_and_rest(f32x4 v, typename Mma<T>::x4& hi, typename Mma<T>::x4& lo) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float x = v[e];
+        asm("" : "+v"(x));
+        v[e] = x;
+    }
+    hi = round4<T>(v);
+    if constexpr (sizeof(T) == 2 && !std::is_same_v<T, _Float16>) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const T top = hi[e];
+            const int left = static_cast<int>(__float_as_uint(v[e]) -
+                                              (static_cast<uint32_t>(__builtin_bit_cast(unsigned short, top)) << 16));
+            lo[e] = __builtin_bit_cast(T, static_cast<short>(left < 0x7fff ? left : 0x7fff));
+        }
+    } else {
+        lo = round4<T>(v - wide4<T>(hi));
+    }
+}
+template <typename T>
+__device__ __forceinline__ float with_rest(T hi, T lo) {
+    if constexpr (sizeof(T) == 2 && !std::is_same_v<T, _Float16>) {
+        const uint32_t top = static_cast<uint32_t>(__builtin_bit_cast(unsigned short, hi)) << 16;
+        return __uint_as_float(top + static_cast<uint32_t>(static_cast<int>(__builtin_bit_cast(short, lo))));
+    } else {
+        return static_cast<float>(hi) + static_cast<float>(lo);
+    }
 }
 
 // The lane's A fragment of the transpose of rows row0 .. row0 + 15 at columns

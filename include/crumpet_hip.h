@@ -438,10 +438,13 @@ CRUMPET_API int crumpet_bucket_bias_backward(void* grad_table, const void* grad,
  *
  * For the backward pass the forward pass also writes row_max and row_inv [B,
  * heads, N] (the softmax statistics, for a backward pass with the same
- * arguments; both may be NULL otherwise) and, for 16-bit types, out_rest like out: what out's rounding
- * left, so that the row sums dO . out, which enter the fp32 gradient of the
- * bias, are those of the unrounded output.  grad_bias [heads, N, N] fp32 or
- * NULL.  workspace: crumpet_window_attention_workspace bytes, 16-byte aligned.
+ * arguments; both may be NULL otherwise) and, for 16-bit types, out_rest, a
+ * dense [B, N, C] of 16 bits each: what out's rounding left, so that the row
+ * sums dO . out, which enter the fp32 gradient of the bias, are those of the
+ * unrounded output (float16: the rest rounded to float16; bfloat16: the bits
+ * of fp32 below out's, as a signed whole number).  grad_bias [heads, N, N]
+ * fp32 or NULL.  workspace: crumpet_window_attention_workspace bytes, 16-byte
+ * aligned.
  *
  * No counterpart in the reference, which is forward-only (README.md:152).
  */

@@ -120,6 +120,31 @@ def test_sharp_and_flat_scores(dev, dtype):
     ref.check(_run(dev, flat, 0 * bias, 2, g), ref.window_attention(flat, 0 * bias, 2, g))
 
 
+@pytest.mark.parametrize("dtype", HALF, ids=str)
+@pytest.mark.parametrize("N,D", [(80, 16), (80, 32), (80, 64), (600, 16)])
+def test_the_kept_rest_belongs_to_the_output(dev, dtype, N, D):
+    """With equal scores every weight is exactly 1 and out + rest the mean of v:
+    the sum is off by at most (N + 1) 2^-23 of the mean magnitude, its product
+    with 1/N by 2^-22 of itself (reciprocal and product), the rest by half a
+    step of fp16 (or a step of fp32's, which bf16 keeps as bits).  The sums of many windows hold means near a tie of the
+    output's rounding, where a rest that belongs to the other neighbour is a
+    whole step off."""
+    qkv = seeded((90, N, 3 * D), dtype, 7)
+    qkv[..., :2 * D] = 0
+    bias = torch.zeros(1, N, N, device=dev)
+    out, rest, _, _ = torch.ops.crumpet_ops.window_attention_forward(qkv.to(dev), bias, 1, None, [], D ** -0.5)
+    v = qkv[..., 2 * D:].double()
+    mean, size = v.mean(1, keepdim=True), v.abs().mean(1, keepdim=True)
+    out, rest = out.cpu(), rest.cpu()
+    if dtype == torch.bfloat16:
+        bits = (out.view(torch.int16).int() << 16) + rest.view(torch.int16).int()
+        both, kept = bits.view(torch.float32).double(), 2.0 ** -23
+    else:
+        both, kept = out.double() + rest.double(), 2.0 ** -22
+    bound = (N + 1) * 2.0 ** -23 * size + (2.0 ** -22 + kept) * mean.abs() + 2.0 ** -25
+    assert ((both - mean).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.5, 2.0 ** -30, 3.0])
 def test_scales(dev, scale):
     qkv, bias, g = _inputs(2, 70, 2, 16, torch.bfloat16)
