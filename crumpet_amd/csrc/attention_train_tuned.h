@@ -248,17 +248,46 @@ __device__ __forceinline__ void settled(V& v) {
     asm volatile("" : "+v"(v));
 }
 
+// Four neighbours that lie anywhere (rows of an odd length): one load.
+template <typename E>
+struct __attribute__((packed)) Neighbours {
+    E v[4];
+};
+
+// from[at + r] for the 4 values from `other`, those past N the last one's.
+// kWhole: all 16 of the tile's are below N.
+template <bool kWhole, typename E>
+__device__ __forceinline__ f32x4 along(const E* row, int other, int N) {
+    f32x4 v;
+    if constexpr (kWhole) {
+        const Neighbours<E> n = *reinterpret_cast<const Neighbours<E>*>(row + other);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = static_cast<float>(n.v[r]);
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = static_cast<float>(row[other + r < N ? other + r : N - 1]);
+    }
+    return v;
+}
+
 template <int NT, bool kKeysInLanes, typename M>
 __device__ __forceinline__ void add_mask(f32x4* tile, const M* mask, int N, int mine, int first) {
     asm volatile("" : "+v"(mine), "+v"(first));
+    const int tile0 = __builtin_amdgcn_readfirstlane(first) & ~15;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
+        if constexpr (kKeysInLanes) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int other = 16 * t + first + r, o = other < N ? other : N - 1;
-            tile[t][r] += static_cast<float>(mask[kKeysInLanes ? o * N + mine : mine * N + o]);
+            for (int r = 0; r < 4; ++r) {
+                const int other = 16 * t + first + r, o = other < N ? other : N - 1;
+                tile[t][r] += static_cast<float>(mask[o * N + mine]);
+            }
+            tiles_in_order();
+        } else {
+            const M* row = mask + mine * N;
+            tile[t] += tile0 + 16 * t + 16 <= N ? along<true>(row, 16 * t + first, N) : along<false>(row, 16 * t + first, N);
+            if (t % 4 == 3) tiles_in_order();
         }
-        tiles_in_order();
     }
 }
 
@@ -274,14 +303,27 @@ __device__ __forceinline__ void build_tiles(f32x4* tile, const AttnArgs& a, int 
     // keeps the addresses of all tiles from being computed ahead of the walk
     // and held in registers through it
     asm volatile("" : "+v"(mine), "+v"(first));
+    const int tile0 = __builtin_amdgcn_readfirstlane(first) & ~15;
+    const float* row = bias + mine * a.N;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
+        // With a mask tensor four tiles' rows are on their way at once: its
+        // kinds are many and their windows few.  (Without one the branches
+        // cost registers that the folded kernels do not have.)
+        if constexpr (kMask && !kKeysInLanes) {
+            if (t % 4 == 0) {
+#pragma unroll
+                for (int u = t; u < t + 4 && u < NT; ++u)
+                    tile[u] = tile0 + 16 * u + 16 <= a.N ? along<true>(row, 16 * u + first, a.N)
+                                                         : along<false>(row, 16 * u + first, a.N);
+            }
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int other = 16 * t + first + r;
             const bool in = other < a.N;
             const int o = in ? other : a.N - 1;
-            float v = bias[kKeysInLanes ? o * a.N + mine : mine * a.N + o];
+            float v = kKeysInLanes ? bias[o * a.N + mine] : kMask ? tile[t][r] : row[o];
             if constexpr (!kMask) {
                 if ((side[o] ^ side[mine]) & kind) v -= 100.0f;
                 v *= per_scale;
