@@ -41,7 +41,8 @@ int64_t rounded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 bool use_tuned(const AttnArgs& a, int32_t dtype, int64_t D) {
     if (a.st < 0 || a.st >= int64_t(1) << 21 || a.H > 4096) return false;
     const bool folds = a.scale >= 0x1p-20f && a.scale <= 0x1p20f;
-    return dtype != CRUMPET_DTYPE_F32 && (D == 16 || D == 32) && a.N <= 512 && (folds || a.mode == kTensorMask);
+    return dtype != CRUMPET_DTYPE_F32 && (D == 16 || D == 32) && a.N <= 512 &&
+           (a.mode == kTensorMask ? a.N >= 2 : folds);  // four neighbours of a mask matrix are read at once
 }
 
 int check(AttnArgs& a, int32_t dtype, int64_t B, int64_t H, int64_t N, int64_t D, const int64_t strides[2],

@@ -250,44 +250,64 @@ __device__ __forceinline__ void settled(V& v) {
 
 // Four neighbours that lie anywhere (rows of an odd length): one load.
 template <typename E>
-struct __attribute__((packed)) Neighbours {
+struct __attribute__((packed, aligned(sizeof(E)))) Neighbours {
     E v[4];
 };
 
-// from[at + r] for the 4 values from `other`, those past N the last one's.
-// kWhole: all 16 of the tile's are below N.
-template <bool kWhole, typename E>
-__device__ __forceinline__ f32x4 along(const E* row, int other, int N) {
-    f32x4 v;
-    if constexpr (kWhole) {
-        const Neighbours<E> n = *reinterpret_cast<const Neighbours<E>*>(row + other);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = static_cast<float>(n.v[r]);
-    } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = static_cast<float>(row[other + r < N ? other + r : N - 1]);
-    }
-    return v;
-}
-
-template <int NT, bool kKeysInLanes, typename M>
-__device__ __forceinline__ void add_mask(f32x4* tile, const M* mask, int N, int mine, int first) {
+// bias + mask for a lane whose rows are keys, -inf past N (N >= 2).  All rows
+// of the bias are on their way at once, straight into the tiles, and the mask's
+// 6 tiles at a time.  A read may run into the next query's row, never past
+// the matrix: the last query's last keys are read singly afterwards.
+template <int NT, typename M>
+__device__ __forceinline__ void add_rows(f32x4* tile, const float* bias, const M* mask, int N, int mine, int first) {
     asm volatile("" : "+v"(mine), "+v"(first));
-    const int tile0 = __builtin_amdgcn_readfirstlane(first) & ~15;
+    const uint32_t row = static_cast<uint32_t>(mine * N + first), last = static_cast<uint32_t>(N * N - 4);
+    const auto place = [&](int t) { return row + 16 * t < last ? row + 16 * t : last; };
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        if constexpr (kKeysInLanes) {
+        const Neighbours<float> b = *reinterpret_cast<const Neighbours<float>*>(bias + place(t));
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int other = 16 * t + first + r, o = other < N ? other : N - 1;
-                tile[t][r] += static_cast<float>(mask[o * N + mine]);
-            }
-            tiles_in_order();
-        } else {
-            const M* row = mask + mine * N;
-            tile[t] += tile0 + 16 * t + 16 <= N ? along<true>(row, 16 * t + first, N) : along<false>(row, 16 * t + first, N);
-            if (t % 4 == 3) tiles_in_order();
+        for (int r = 0; r < 4; ++r) tile[t][r] = b.v[r];
+    }
+    tiles_in_order();
+#pragma unroll
+    for (int t0 = 0; t0 < NT; t0 += 6) {
+        Neighbours<M> m[6];
+#pragma unroll
+        for (int u = 0; u < 6 && t0 + u < NT; ++u)
+            m[u] = *reinterpret_cast<const Neighbours<M>*>(mask + place(t0 + u));
+#pragma unroll
+        for (int u = 0; u < 6 && t0 + u < NT; ++u) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                tile[t0 + u][r] = 16 * (t0 + u) + first + r < N ? tile[t0 + u][r] + static_cast<float>(m[u].v[r])
+                                                                : -__builtin_inff();
         }
+        tiles_in_order();
+    }
+    if (mine + 1 < N) return;
+    asm volatile("" : "+v"(first));
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int at = 16 * t + first;
+        if (at >= N || at + 4 <= N) continue;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (at + r < N) tile[t][r] = bias[mine * N + at + r] + static_cast<float>(mask[mine * N + at + r]);
+    }
+}
+// The same for a lane whose column is a key; rows past N are the last one's.
+template <int NT, typename M>
+__device__ __forceinline__ void add_columns(f32x4* tile, const float* bias, const M* mask, int N, int mine, int first) {
+    asm volatile("" : "+v"(mine), "+v"(first));
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int other = 16 * t + first + r, o = other < N ? other : N - 1;
+            tile[t][r] = bias[o * N + mine] + static_cast<float>(mask[o * N + mine]);
+        }
+        if (t % 2 == 1) tiles_in_order();
     }
 }
 
@@ -303,43 +323,35 @@ __device__ __forceinline__ void build_tiles(f32x4* tile, const AttnArgs& a, int 
     // keeps the addresses of all tiles from being computed ahead of the walk
     // and held in registers through it
     asm volatile("" : "+v"(mine), "+v"(first));
-    const int tile0 = __builtin_amdgcn_readfirstlane(first) & ~15;
-    const float* row = bias + mine * a.N;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        // With a mask tensor four tiles' rows are on their way at once: its
-        // kinds are many and their windows few.  (Without one the branches
-        // cost registers that the folded kernels do not have.)
-        if constexpr (kMask && !kKeysInLanes) {
-            if (t % 4 == 0) {
-#pragma unroll
-                for (int u = t; u < t + 4 && u < NT; ++u)
-                    tile[u] = tile0 + 16 * u + 16 <= a.N ? along<true>(row, 16 * u + first, a.N)
-                                                         : along<false>(row, 16 * u + first, a.N);
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int other = 16 * t + first + r;
-            const bool in = other < a.N;
-            const int o = in ? other : a.N - 1;
-            float v = kKeysInLanes ? bias[o * a.N + mine] : kMask ? tile[t][r] : row[o];
-            if constexpr (!kMask) {
-                if ((side[o] ^ side[mine]) & kind) v -= 100.0f;
-                v *= per_scale;
-            }
-            tile[t][r] = in || kKeysInLanes ? v : -__builtin_inff();
-        }
-        tiles_in_order();
-    }
     if constexpr (kMask) {
         const int64_t at = static_cast<int64_t>(kind) * a.mask_sb;
+        const auto add = [&](auto mask) {
+            if constexpr (kKeysInLanes)
+                add_columns<NT>(tile, bias, mask + at, a.N, mine, first);
+            else
+                add_rows<NT>(tile, bias, mask + at, a.N, mine, first);
+        };
         if (a.mask_dtype == CRUMPET_DTYPE_F32)
-            add_mask<NT, kKeysInLanes>(tile, static_cast<const float*>(a.mask) + at, a.N, mine, first);
+            add(static_cast<const float*>(a.mask));
         else if (a.mask_dtype == CRUMPET_DTYPE_F16)
-            add_mask<NT, kKeysInLanes>(tile, static_cast<const _Float16*>(a.mask) + at, a.N, mine, first);
+            add(static_cast<const _Float16*>(a.mask));
         else
-            add_mask<NT, kKeysInLanes>(tile, static_cast<const __bf16*>(a.mask) + at, a.N, mine, first);
+            add(static_cast<const __bf16*>(a.mask));
+    } else {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int other = 16 * t + first + r;
+                const bool in = other < a.N;
+                const int o = in ? other : a.N - 1;
+                float v = bias[kKeysInLanes ? o * a.N + mine : mine * a.N + o];
+                if ((side[o] ^ side[mine]) & kind) v -= 100.0f;
+                v *= per_scale;
+                tile[t][r] = in || kKeysInLanes ? v : -__builtin_inff();
+            }
+            tiles_in_order();
+        }
     }
 }
 

@@ -97,6 +97,17 @@ def test_mask_tensors(dev, dtype, D, mask_dtype, kind, M, N):
         assert torch.isfinite(found["grad_bias"]).all()
 
 
+@pytest.mark.parametrize("dtype,D,mask_dtype", [(torch.float16, 16, torch.float16), (torch.bfloat16, 32, torch.bfloat16),
+                                                (torch.float16, 32, torch.float32)], ids=str)
+@pytest.mark.parametrize("N", [1, 2, 3, 4, 5, 15, 16, 18, 47, 48, 65, 127, 226, 349, 350, 352, 511, 512])
+def test_mask_rows_read_four_at_a_time(dev, dtype, D, mask_dtype, N):
+    """Rows of odd and even lengths, ends inside and at the end of a group of
+    four, the last row's at the end of the mask's and the bias' memory."""
+    mask = _mask(2, N, "hundred", mask_dtype)
+    qkv, bias, g = _inputs(4, N, 2, D, dtype, seed=N)
+    ref.check(_run(dev, qkv, bias, 2, g, mask=mask), ref.window_attention(qkv, bias, 2, g, mask))
+
+
 @pytest.mark.parametrize("dtype", ALL, ids=str)
 def test_a_nan_stays_in_its_window_and_head(dev, dtype):
     qkv, bias, g = _inputs(3, 40, 2, 16, dtype)
