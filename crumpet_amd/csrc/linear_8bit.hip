@@ -18,6 +18,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "crumpet_common.h"
 #include "crumpet_hip.h"
@@ -36,40 +37,54 @@ __device__ __forceinline__ float power_of_two(int e) {
     return e == kNaN ? __builtin_nanf("") : __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
 
-// The normal distribution Phi(x) = erfc(-x / sqrt 2) / 2 and x times its
-// density.  erfc by formula 7.1.26 of Abramowitz & Stegun, Handbook of
-// Mathematical Functions (|error| <= 1.5e-7, far below a 16-bit result's
-// rounding); the negative side uses erfc itself, so nothing cancels.
-struct Normal {
-    float phi, x_density;
-    __device__ __forceinline__ explicit Normal(float x) {
-        const float z = fabsf(x) * 0.70710678f;
-        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, z, 1.0f));
-        float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-        p = __builtin_fmaf(p, t, 1.421413741f);
-        p = __builtin_fmaf(p, t, -0.284496736f);
-        p = __builtin_fmaf(p, t, 0.254829592f);
-        const float bell = __builtin_amdgcn_exp2f(z * z * -kLog2e);
-        const float half_erfc = 0.5f * p * t * bell;
-        phi = x > 0.0f ? 1.0f - half_erfc : half_erfc;
-        x_density = x * bell * 0.39894228f;
+// GELU(x) = x Phi(x) and its derivative Phi(x) + x phi(x), with the normal
+// distribution from its tail, Phi(-|x|) = erfc(|x| / sqrt 2) / 2 = u(t)
+// exp(-x^2 / 2), t = 1 / (1 + p |x| / sqrt 2): formula 7.1.26 of Abramowitz &
+// Stegun, Handbook of Mathematical Functions (|error| of erfc <= 1.5e-7, far
+// below a 16-bit result's rounding).  The arithmetic of these two bounds the
+// kernels, so it is written for few instructions.
+struct Tail {
+    float u, bell;
+    __device__ __forceinline__ explicit Tail(float x) {
+        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678f, fabsf(x), 1.0f));
+        float p = __builtin_fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+        p = __builtin_fmaf(p, t, 0.5f * 1.421413741f);
+        p = __builtin_fmaf(p, t, 0.5f * -0.284496736f);
+        p = __builtin_fmaf(p, t, 0.5f * 0.254829592f);
+        u = p * t;
+        bell = __builtin_amdgcn_exp2f(x * x * (-0.5f * kLog2e));
     }
 };
 template <bool kGelu>
 __device__ __forceinline__ float act(float x) {
-    if constexpr (kGelu) return x * Normal(x).phi;
+    if constexpr (kGelu) {
+        const Tail n(x);
+        const float low = n.u * n.bell;
+        return x * (x > 0.0f ? 1.0f - low : low);
+    }
     return x;
 }
 template <bool kGelu>
 __device__ __forceinline__ float act_grad(float x) {
     if constexpr (kGelu) {
-        const Normal n(x);
-        return n.phi + n.x_density;
+        // 1/2 +- (1/2 - Phi(-|x|) + |x| phi(x)), phi(x) = bell / sqrt(2 pi)
+        const Tail n(x);
+        return 0.5f + copysignf(__builtin_fmaf(n.bell, __builtin_fmaf(0.39894228f, fabsf(x), -n.u), 0.5f), x);
     }
     return 1.0f;
 }
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// The V at a 32-bit byte offset of the lane's from a base of the workgroup's,
+// which keeps the address out of the lane's arithmetic.
+template <typename V, typename P>
+__device__ __forceinline__ __attribute__((address_space(1))) V& at(P* base, uint32_t bytes) {
+    typedef std::conditional_t<std::is_const_v<P>, const char, char> Byte;
+    typedef __attribute__((address_space(1))) Byte GlobalByte;
+    typedef __attribute__((address_space(1))) V GlobalV;
+    return *(GlobalV*)((GlobalByte*)(base) + bytes);
+}
 
 // Codes of 8 of a group's 32 values (the other lanes of the row hold the
 // rest), and the group's exponent.  Magnitudes compare as their 16 bits, NaN
@@ -138,116 +153,181 @@ struct RowsArgs {
 
 // y = f(x) w^T.  Forward: f = act, the bias added, codes written by the first
 // column block.  Backward (x = dy, w = W^T): y times act' of the codes at y's
-// place.  A wave owns 32 rows, a workgroup 128 rows and 16 NT columns.
+// place.  A wave owns 32 rows, a workgroup 128 rows and 16 NT columns; all
+// addresses are a base of the workgroup's and a 32-bit offset of the lane's
+// that the loops leave alone.
 template <typename T, int NT, bool kGelu, bool kForward>
 __global__ void __launch_bounds__(kThreads) linear_8bit_rows_kernel(const RowsArgs a, uint32_t row_blocks, uint32_t blocks) {
+    typedef typename Mma<T>::x4 X4;
     typedef typename Mma<T>::x8 X8;
     uint32_t id;
     if (!xcd_chunk(blockIdx.x, gridDim.x, row_blocks * blocks, id)) return;
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
     const int n0 = static_cast<int>(id % blocks) * 16 * NT;
-    const int64_t row0 = static_cast<int64_t>(id / blocks) * 128 + (threadIdx.x >> 6) * 32 + col;
+    const int64_t block0 = static_cast<int64_t>(id / blocks) * 128;
+    const int row0 = (threadIdx.x >> 6) * 32 + col;
+    const int rows = static_cast<int>(std::min<int64_t>(128, a.rows - block0));
     const int groups = (a.K + kGroup - 1) / kGroup;
     const bool keep = kForward && n0 == 0 && a.codes != nullptr;
-    const T* xr[2];
-    int64_t row[2];
+    const T* x_at = static_cast<const T*>(a.x) + block0 * a.K;
+    const T* w_at = static_cast<const T*>(a.w) + static_cast<int64_t>(n0) * a.K;
+    uint32_t x_of[2], w_of[NT];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        row[r] = row0 + 16 * r;
-        xr[r] = static_cast<const T*>(a.x) + (row[r] < a.rows ? row[r] : a.rows - 1) * a.K;
-    }
+    for (int r = 0; r < 2; ++r) x_of[r] = (std::min(row0 + 16 * r, rows - 1) * a.K + 8 * g) * sizeof(T);
     // Row m of tile n is feature 4 NT (m / 4) + 4 n + m % 4 of the block, so that
     // a lane ends with 4 NT neighbouring features of its row.
-    const T* wr[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int f = n0 + 4 * NT * (col >> 2) + 4 * n + (col & 3);
-        wr[n] = static_cast<const T*>(a.w) + static_cast<int64_t>(f < a.n_out ? f : a.n_out - 1) * a.K;
-    }
-    // K is a multiple of 16: the last step may be half a group
-    X8 xv[2], wv[NT];
-    const auto fetch = [&](int k0) {
-        const int k = k0 + 8 * g;
-        const bool in = k < a.K;
+    for (int n = 0; n < NT; ++n) 
+        w_of[n] = (std::min(4 * NT * (col >> 2) + 4 * n + (col & 3), a.n_out - 1 - n0) * a.K + 8 * g) * sizeof(T);
+    const int out_groups = (a.n_out + kGroup - 1) / kGroup;
+    const int f0 = 4 * NT * g;  // the lane's features, from n0
+    T* y_at = static_cast<T*>(a.y) + block0 * a.n_out + n0;
+    // two tiles are 8 neighbouring features of one group: 16 bytes, aligned where
+    // NT is even
+    constexpr int kEach = NT % 2 == 0 ? 2 : 1;
+    const auto place = [&](int n, int r) { return static_cast<uint32_t>((row0 + 16 * r) * a.n_out + f0 + 4 * n); };
+    // the backward pass' codes, on their way while the products are formed
+    uint32_t codes[NT][2] = {};
+    int8_t exps[NT][2] = {};
+    if constexpr (!kForward && kGelu) {
+        const int8_t* codes_at = a.codes + block0 * a.n_out + n0;
+        const int8_t* exps_at = a.exps + block0 * out_groups;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            xv[r] = X8{};
-            if (in) xv[r] = *reinterpret_cast<const X8*>(xr[r] + k);
+        for (int n = 0; n < NT; n += kEach) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                if (row0 + 16 * r >= rows || n0 + f0 + 4 * n >= a.n_out) continue;
+                exps[n][r] = at<const int8_t>(exps_at, (row0 + 16 * r) * out_groups + (n0 + f0 + 4 * n) / kGroup);
+                if constexpr (kEach == 2) {
+                    if (n0 + f0 + 4 * n + 4 < a.n_out) {
+                        const u32x2 both = at<const u32x2>(codes_at, place(n, r));
+                        codes[n][r] = both[0], codes[n + 1][r] = both[1];
+                        continue;
+                    }
+                }
+                codes[n][r] = at<const uint32_t>(codes_at, place(n, r));
+            }
         }
+    }
+    // Two groups a step, so that a row's 128-byte lines are read at once.  x is
+    // requested a step ahead; the weights, which stay in L2, at the start of
+    // their step.  K is a multiple of 16: the last step may be short.
+    X8 xv[2][2];
+    const auto fetch = [&](int k0) {
+        // a new scalar base each time, not a vector pointer that is advanced
+        asm volatile("" : "+s"(x_at));
+        if (k0 + 2 * kGroup <= a.K) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            wv[n] = X8{};
-            if (in) wv[n] = *reinterpret_cast<const X8*>(wr[n] + k);
+            for (int r = 0; r < 2; ++r) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s) xv[s][r] = at<const X8>(x_at + k0 + s * kGroup, x_of[r]);
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    xv[s][r] = X8{};
+                    if (k0 + s * kGroup + 8 * g < a.K) xv[s][r] = at<const X8>(x_at + k0 + s * kGroup, x_of[r]);
+                }
+            }
         }
     };
     f32x4 acc[NT][2] = {};
     fetch(0);
-    for (int k0 = 0; k0 < a.K; k0 += kGroup) {
-        X8 x[2] = {xv[0], xv[1]}, w[NT];
+    for (int k0 = 0; k0 < a.K; k0 += 2 * kGroup) {
+        const bool both = k0 + kGroup < a.K;
+        X8 x[2][2], w[2][NT];
+        asm volatile("" : "+s"(w_at));
+        if (k0 + 2 * kGroup <= a.K) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) w[n] = wv[n];
-        if (k0 + kGroup < a.K) fetch(k0 + kGroup);
-        if constexpr (kForward) {
-            const int k = k0 + 8 * g;
+            for (int s = 0; s < 2; ++s) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+                for (int n = 0; n < NT; ++n) w[s][n] = at<const X8>(w_at + k0 + s * kGroup, w_of[n]);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    w[s][n] = X8{};
+                    if (k0 + s * kGroup + 8 * g < a.K) w[s][n] = at<const X8>(w_at + k0 + s * kGroup, w_of[n]);
+                }
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) x[s][0] = xv[s][0], x[s][1] = xv[s][1];
+        if (k0 + 2 * kGroup < a.K) fetch(k0 + 2 * kGroup);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            if (s == 1 && !both) break;
+            const int k = k0 + s * kGroup;
+            if constexpr (kForward) {
                 if (keep) {
-                    int e;
-                    const u32x2 codes = quantise<T>(x[r], e);
-                    if (row[r] < a.rows) {
-                        if (k < a.K) *reinterpret_cast<u32x2*>(a.codes + row[r] * a.K + k) = codes;
-                        if (g == 0) a.exps[row[r] * groups + k0 / kGroup] = static_cast<int8_t>(e);
+                    int8_t* codes_at = a.codes + block0 * a.K + k;
+                    int8_t* exps_at = a.exps + block0 * groups + k / kGroup;
+                    asm volatile("" : "+s"(codes_at), "+s"(exps_at));
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        int e;
+                        const u32x2 codes = quantise<T>(x[s][r], e);
+                        if (row0 + 16 * r < rows) {
+                            if (k + 8 * g < a.K) at<u32x2>(codes_at, x_of[r] / sizeof(T)) = codes;
+                            if (g == 0) at<int8_t>(exps_at, (row0 + 16 * r) * groups) = static_cast<int8_t>(e);
+                        }
                     }
                 }
                 if constexpr (kGelu) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[r][i] = static_cast<T>(act<true>(static_cast<float>(x[r][i])));
+                    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) x[s][r][i] = static_cast<T>(act<true>(static_cast<float>(x[s][r][i])));
+                    }
                 }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) acc[n][r] = Mma<T>::mma32(w[s][n], x[s][r], acc[n][r]);
+            }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; n += kEach) {
+        if (n0 + f0 + 4 * n >= a.n_out) continue;
+        const bool pair = kEach == 2 && n0 + f0 + 4 * n + 4 < a.n_out;
+        f32x4 b[kEach] = {};
+        if constexpr (kForward) {
+            if (a.b != nullptr) {
+                const T* b_at = static_cast<const T*>(a.b) + n0;
+                b[0] = wide4<T>(at<const X4>(b_at, (f0 + 4 * n) * sizeof(T)));
+                if constexpr (kEach == 2)
+                    if (pair) b[1] = wide4<T>(at<const X4>(b_at, (f0 + 4 * n + 4) * sizeof(T)));
             }
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int r = 0; r < 2; ++r) acc[n][r] = Mma<T>::mma32(w[n], x[r], acc[n][r]);
-        }
-    }
-    const int out_groups = (a.n_out + kGroup - 1) / kGroup;
-    const int f0 = n0 + 4 * NT * g;
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        if (row[r] >= a.rows) continue;
-        T* to = static_cast<T*>(a.y) + row[r] * a.n_out + f0;
-        // two tiles are 8 neighbouring features: 16 bytes, aligned where NT is even
-#pragma unroll
-        for (int n = 0; n < NT; n += NT % 2 == 0 ? 2 : 1) {
-            constexpr int kEach = NT % 2 == 0 ? 2 : 1;
+        for (int r = 0; r < 2; ++r) {
+            if (row0 + 16 * r >= rows) continue;
             f32x4 v[kEach];
-            bool in[kEach];
 #pragma unroll
-            for (int u = 0; u < kEach; ++u) {
-                const int f = f0 + 4 * (n + u);
-                in[u] = f < a.n_out;
-                v[u] = acc[n + u][r];
-                if (!in[u]) continue;
-                if constexpr (kForward) {
-                    if (a.b != nullptr) v[u] += wide4<T>(load4<T>(static_cast<const T*>(a.b) + f));
-                } else if constexpr (kGelu) {
-                    const f32x4 x = values_of(*reinterpret_cast<const uint32_t*>(a.codes + row[r] * a.n_out + f),
-                                              power_of_two(a.exps[row[r] * out_groups + f / kGroup]));
+            for (int u = 0; u < kEach; ++u) v[u] = acc[n + u][r] + b[u];
+            if constexpr (!kForward && kGelu) {
+                const float step = power_of_two(exps[n][r]);
+#pragma unroll
+                for (int u = 0; u < kEach; ++u) {
+                    const f32x4 x = values_of(codes[n + u][r], step);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) v[u][i] *= act_grad<true>(x[i]);
                 }
             }
+            const X4 lo = round4<T>(v[0]);
             if constexpr (kEach == 2) {
-                if (in[1]) {
-                    const typename Mma<T>::x4 lo = round4<T>(v[0]), hi = round4<T>(v[1]);
-                    *reinterpret_cast<X8*>(to + 4 * n) = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                if (pair) {
+                    at<X8>(y_at, place(n, r) * sizeof(T)) = __builtin_shufflevector(lo, round4<T>(v[1]), 0, 1, 2, 3, 4, 5, 6, 7);
                     continue;
                 }
             }
-#pragma unroll
-            for (int u = 0; u < kEach; ++u)
-                if (in[u]) *reinterpret_cast<typename Mma<T>::x4*>(to + 4 * (n + u)) = round4<T>(v[u]);
+            at<X4>(y_at, place(n, r) * sizeof(T)) = lo;
         }
     }
 }
