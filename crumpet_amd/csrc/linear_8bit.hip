@@ -151,34 +151,67 @@ struct RowsArgs {
     int32_t K, n_out;
 };
 
+constexpr int kStep = 2 * kGroup;  // columns of a step
+
+// A step's weights in LDS: row 16 n + m is feature 4 NT (m / 4) + 4 n + m % 4 of
+// the block, so that a lane ends with 4 NT neighbouring features of its row.
+// The 16-byte pieces of a row are permuted by it, so that 8 lanes of a fragment
+// read meet distinct banks.  Straight from memory: load j fills rows 8 j .. + 7.
+template <typename T, int NT>
+struct Weights {
+    static constexpr int kEach = (2 * NT + 3) / 4;
+    const T* first;
+    uint32_t bytes;
+    int wave, piece, row[kEach];
+    __device__ __forceinline__ Weights(const RowsArgs& a, int n0, int lane) {
+        wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+        first = static_cast<const T*>(a.w) + static_cast<int64_t>(n0) * a.K;
+        const int features = std::min(16 * NT, a.n_out - n0);
+        bytes = static_cast<uint32_t>(features) * a.K * sizeof(T);
+        piece = ((lane & 7) ^ (lane >> 3)) * 8;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int at = 8 * (wave + 4 * i) + (lane >> 3), n = at >> 4, m = at & 15;
+            row[i] = std::min(4 * NT * (m >> 2) + 4 * n + (m & 3), features - 1) * a.K;
+        }
+    }
+    __device__ __forceinline__ void load(const RowsArgs& a, T* to, int k0) const {
+        const u32x4 buffer = buffer_of(first, bytes);
+        const uint32_t lds = lds_address(to);
+        const int k = std::min(k0 + piece, a.K - 8);  // a short step's pieces past K: some other of the row
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (wave + 4 * i < 2 * NT) load_to_lds(buffer, lds + (wave + 4 * i) * 1024, (row[i] + k) * sizeof(T));
+    }
+    static __device__ __forceinline__ int fragment(int s, int n, int col, int g) {
+        return (16 * n + col) * kStep + ((4 * s + g) ^ (col & 7)) * 8;
+    }
+};
+
 // y = f(x) w^T.  Forward: f = act, the bias added, codes written by the first
 // column block.  Backward (x = dy, w = W^T): y times act' of the codes at y's
-// place.  A wave owns 32 rows, a workgroup 128 rows and 16 NT columns; all
+// place.  A wave owns 16 R rows, a workgroup 64 R rows and 16 NT columns; all
 // addresses are a base of the workgroup's and a 32-bit offset of the lane's
 // that the loops leave alone.
-template <typename T, int NT, bool kGelu, bool kForward>
+template <typename T, int NT, int R, bool kGelu, bool kForward>
 __global__ void __launch_bounds__(kThreads) linear_8bit_rows_kernel(const RowsArgs a, uint32_t row_blocks, uint32_t blocks) {
     typedef typename Mma<T>::x4 X4;
     typedef typename Mma<T>::x8 X8;
+    __shared__ __attribute__((aligned(16))) T w_lds[2][NT * 16 * kStep];
     uint32_t id;
     if (!xcd_chunk(blockIdx.x, gridDim.x, row_blocks * blocks, id)) return;
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
     const int n0 = static_cast<int>(id % blocks) * 16 * NT;
-    const int64_t block0 = static_cast<int64_t>(id / blocks) * 128;
-    const int row0 = (threadIdx.x >> 6) * 32 + col;
-    const int rows = static_cast<int>(std::min<int64_t>(128, a.rows - block0));
+    const int64_t block0 = static_cast<int64_t>(id / blocks) * 64 * R;
+    const int row0 = (threadIdx.x >> 6) * 16 * R + col;
+    const int rows = static_cast<int>(std::min<int64_t>(64 * R, a.rows - block0));
     const int groups = (a.K + kGroup - 1) / kGroup;
     const bool keep = kForward && n0 == 0 && a.codes != nullptr;
     const T* x_at = static_cast<const T*>(a.x) + block0 * a.K;
-    const T* w_at = static_cast<const T*>(a.w) + static_cast<int64_t>(n0) * a.K;
-    uint32_t x_of[2], w_of[NT];
+    uint32_t x_of[R];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) x_of[r] = (std::min(row0 + 16 * r, rows - 1) * a.K + 8 * g) * sizeof(T);
-    // Row m of tile n is feature 4 NT (m / 4) + 4 n + m % 4 of the block, so that
-    // a lane ends with 4 NT neighbouring features of its row.
-#pragma unroll
-    for (int n = 0; n < NT; ++n) 
-        w_of[n] = (std::min(4 * NT * (col >> 2) + 4 * n + (col & 3), a.n_out - 1 - n0) * a.K + 8 * g) * sizeof(T);
+    for (int r = 0; r < R; ++r) x_of[r] = (std::min(row0 + 16 * r, rows - 1) * a.K + 8 * g) * sizeof(T);
+    Weights<T, NT> weights(a, n0, lane);
     const int out_groups = (a.n_out + kGroup - 1) / kGroup;
     const int f0 = 4 * NT * g;  // the lane's features, from n0
     T* y_at = static_cast<T*>(a.y) + block0 * a.n_out + n0;
@@ -187,15 +220,15 @@ __global__ void __launch_bounds__(kThreads) linear_8bit_rows_kernel(const RowsAr
     constexpr int kEach = NT % 2 == 0 ? 2 : 1;
     const auto place = [&](int n, int r) { return static_cast<uint32_t>((row0 + 16 * r) * a.n_out + f0 + 4 * n); };
     // the backward pass' codes, on their way while the products are formed
-    uint32_t codes[NT][2] = {};
-    int8_t exps[NT][2] = {};
+    uint32_t codes[NT][R] = {};
+    int8_t exps[NT][R] = {};
     if constexpr (!kForward && kGelu) {
         const int8_t* codes_at = a.codes + block0 * a.n_out + n0;
         const int8_t* exps_at = a.exps + block0 * out_groups;
 #pragma unroll
         for (int n = 0; n < NT; n += kEach) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < R; ++r) {
                 if (row0 + 16 * r >= rows || n0 + f0 + 4 * n >= a.n_out) continue;
                 exps[n][r] = at<const int8_t>(exps_at, (row0 + 16 * r) * out_groups + (n0 + f0 + 4 * n) / kGroup);
                 if constexpr (kEach == 2) {
@@ -209,22 +242,23 @@ __global__ void __launch_bounds__(kThreads) linear_8bit_rows_kernel(const RowsAr
             }
         }
     }
-    // Two groups a step, so that a row's 128-byte lines are read at once.  x is
-    // requested a step ahead; the weights, which stay in L2, at the start of
-    // their step.  K is a multiple of 16: the last step may be short.
-    X8 xv[2][2];
+    // Two groups a step, so that a row's 128-byte lines are read at once, x and
+    // the weights a step ahead.  K is a multiple of 16: the last step may be
+    // short.
+    X8 xv[2][R];
     const auto fetch = [&](int k0) {
+        weights.load(a, w_lds[k0 / kStep & 1], k0);
         // a new scalar base each time, not a vector pointer that is advanced
         asm volatile("" : "+s"(x_at));
-        if (k0 + 2 * kGroup <= a.K) {
+        if (k0 + kStep <= a.K) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < R; ++r) {
 #pragma unroll
                 for (int s = 0; s < 2; ++s) xv[s][r] = at<const X8>(x_at + k0 + s * kGroup, x_of[r]);
             }
         } else {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < R; ++r) {
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
                     xv[s][r] = X8{};
@@ -233,42 +267,30 @@ __global__ void __launch_bounds__(kThreads) linear_8bit_rows_kernel(const RowsAr
             }
         }
     };
-    f32x4 acc[NT][2] = {};
+    f32x4 acc[NT][R] = {};
     fetch(0);
-    for (int k0 = 0; k0 < a.K; k0 += 2 * kGroup) {
-        const bool both = k0 + kGroup < a.K;
-        X8 x[2][2], w[2][NT];
-        asm volatile("" : "+s"(w_at));
-        if (k0 + 2 * kGroup <= a.K) {
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) w[s][n] = at<const X8>(w_at + k0 + s * kGroup, w_of[n]);
-            }
-        } else {
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    w[s][n] = X8{};
-                    if (k0 + s * kGroup + 8 * g < a.K) w[s][n] = at<const X8>(w_at + k0 + s * kGroup, w_of[n]);
-                }
-            }
-        }
-#pragma unroll
-        for (int s = 0; s < 2; ++s) x[s][0] = xv[s][0], x[s][1] = xv[s][1];
-        if (k0 + 2 * kGroup < a.K) fetch(k0 + 2 * kGroup);
+    for (int k0 = 0; k0 < a.K; k0 += kStep) {
+        wait_vmem();
+        __syncthreads();
+        X8 x[2][R];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            if (s == 1 && !both) break;
-            const int k = k0 + s * kGroup;
-            if constexpr (kForward) {
-                if (keep) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) x[s][r] = xv[s][r];
+        }
+        if constexpr (kForward) {
+            // before the next step's loads, so that the wait for them does not
+            // begin with these stores
+            if (keep) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const int k = k0 + s * kGroup;
+                    if (k >= a.K) break;
                     int8_t* codes_at = a.codes + block0 * a.K + k;
                     int8_t* exps_at = a.exps + block0 * groups + k / kGroup;
                     asm volatile("" : "+s"(codes_at), "+s"(exps_at));
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
+                    for (int r = 0; r < R; ++r) {
                         int e;
                         const u32x2 codes = quantise<T>(x[s][r], e);
                         if (row0 + 16 * r < rows) {
@@ -277,18 +299,28 @@ __global__ void __launch_bounds__(kThreads) linear_8bit_rows_kernel(const RowsAr
                         }
                     }
                 }
-                if constexpr (kGelu) {
+            }
+        }
+        if (k0 + kStep < a.K) fetch(k0 + kStep);
+        const T* tile = w_lds[k0 / kStep & 1];
+        const bool whole = k0 + kStep <= a.K;
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
+        for (int s = 0; s < 2; ++s) {
+            if (k0 + s * kGroup >= a.K) break;
+            if constexpr (kForward && kGelu) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) x[s][r][i] = static_cast<T>(act<true>(static_cast<float>(x[s][r][i])));
-                    }
+                for (int r = 0; r < R; ++r) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[s][r][i] = static_cast<T>(act<true>(static_cast<float>(x[s][r][i])));
                 }
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
+                X8 w = *reinterpret_cast<const X8*>(tile + weights.fragment(s, n, col, g));
+                // past K lies some other weight, which zeros in x need not silence
+                if (!whole && k0 + s * kGroup + 8 * g >= a.K) w = X8{};
 #pragma unroll
-                for (int r = 0; r < 2; ++r) acc[n][r] = Mma<T>::mma32(w[s][n], x[s][r], acc[n][r]);
+                for (int r = 0; r < R; ++r) acc[n][r] = Mma<T>::mma32(w, x[s][r], acc[n][r]);
             }
         }
     }
@@ -306,7 +338,7 @@ __global__ void __launch_bounds__(kThreads) linear_8bit_rows_kernel(const RowsAr
             }
         }
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+        for (int r = 0; r < R; ++r) {
             if (row0 + 16 * r >= rows) continue;
             f32x4 v[kEach];
 #pragma unroll
@@ -490,17 +522,18 @@ __global__ void __launch_bounds__(kThreads) linear_8bit_join_kernel(T* dw, T* db
     }
 }
 
-template <typename T, bool kGelu, bool kForward>
-int rows_product(const RowsArgs& a, hipStream_t s) {
+template <typename T, int R, bool kGelu, bool kForward>
+int rows_launch(const RowsArgs& a, hipStream_t s) {
+    constexpr int kMost = kForward && kGelu && R == 2 ? 8 : 4;
     const int tiles = a.n_out / 16;
-    const uint32_t row_blocks = static_cast<uint32_t>((a.rows + 127) / 128);
-    // the fewest column blocks of at most 8 tiles, evenly cut
-    const int blocks = (tiles + 7) / 8, nt = (tiles + blocks - 1) / blocks;
+    const uint32_t row_blocks = static_cast<uint32_t>((a.rows + 64 * R - 1) / (64 * R));
+    const int blocks = (tiles + kMost - 1) / kMost, nt = (tiles + blocks - 1) / blocks;
     const uint32_t grid = xcd_launch_count(row_blocks * static_cast<uint32_t>(blocks));
-#define CRUMPET_ROWS(NT)                                                                                          \
-    case NT:                                                                                                      \
-        linear_8bit_rows_kernel<T, NT, kGelu, kForward><<<grid, kThreads, 0, s>>>(a, row_blocks,                  \
-                                                                                  static_cast<uint32_t>(blocks)); \
+#define CRUMPET_ROWS(NT)                                                                                             \
+    case NT:                                                                                                         \
+        if constexpr (NT <= kMost)                                                                                   \
+            linear_8bit_rows_kernel<T, NT, R, kGelu, kForward><<<grid, kThreads, 0, s>>>(                            \
+                a, row_blocks, static_cast<uint32_t>(blocks));                                                       \
         break;
     switch (nt) {
         CRUMPET_ROWS(1) CRUMPET_ROWS(2) CRUMPET_ROWS(3) CRUMPET_ROWS(4) CRUMPET_ROWS(5) CRUMPET_ROWS(6)
@@ -508,6 +541,17 @@ int rows_product(const RowsArgs& a, hipStream_t s) {
     }
 #undef CRUMPET_ROWS
     return check_launch("linear_8bit");
+}
+
+// Rows of a wave: 32, or 16 where the wider grid would leave compute units with
+// fewer than two workgroups and a step's latency is what counts.  Features 1536
+// to 384, no activation: 864 rows 47 us against 27, 6912 rows (162 workgroups) 53
+// against 38; 110592 rows of 384 to 96 (864 workgroups) 51 against 52, and with
+// the GELU, which narrower blocks repeat, 62 against 79.
+template <typename T, bool kGelu, bool kForward>
+int rows_product(const RowsArgs& a, hipStream_t s) {
+    const int64_t wide = (a.rows + 127) / 128 * ((a.n_out + 127) / 128);
+    return wide < 512 ? rows_launch<T, 1, kGelu, kForward>(a, s) : rows_launch<T, 2, kGelu, kForward>(a, s);
 }
 
 struct Split {
