@@ -418,19 +418,32 @@ __global__ void __launch_bounds__(kThreads) linear_8bit_weight_kernel(const Weig
     X8 dy_next[2];
     u32x4 codes_next[2];
     int e_next[2];
+    // addresses: a base of the step's and an offset of the lane's
+    uint32_t dy_of[2], x_of[2], e_of[2];
+    bool dy_in[2], x_in[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int p = threadIdx.x + i * kThreads, r = p >> 3, c = p & 7;
+        dy_of[i] = (r * a.n_out + c * 8) * sizeof(T), dy_in[i] = n0 + c * 8 < a.n_out;
+        x_of[i] = r * a.K + c * 16, x_in[i] = k0 + c * 16 < a.K;
+        e_of[i] = r * groups + c / 2;
+    }
     const auto fetch = [&](int64_t r0) {
+        const T* dy_at = static_cast<const T*>(a.dy) + r0 * a.n_out + n0;
+        const int8_t* x_at = a.codes + r0 * a.K + k0;
+        const int8_t* e_at = a.exps + r0 * groups + k0 / kGroup;
+        asm volatile("" : "+s"(dy_at), "+s"(x_at), "+s"(e_at));
+        const int rows = static_cast<int>(std::min<int64_t>(kRows, end - r0));
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int p = threadIdx.x + i * kThreads, r = p >> 3, c = p & 7;
             dy_next[i] = X8{};
             codes_next[i] = u32x4{};
             e_next[i] = 0;
-            if (r0 + r >= end) continue;
-            if (n0 + c * 8 < a.n_out)
-                dy_next[i] = *reinterpret_cast<const X8*>(static_cast<const T*>(a.dy) + (r0 + r) * a.n_out + n0 + c * 8);
-            if (k0 + c * 16 < a.K) {
-                codes_next[i] = *reinterpret_cast<const u32x4*>(a.codes + (r0 + r) * a.K + k0 + c * 16);
-                e_next[i] = a.exps[(r0 + r) * groups + (k0 + c * 16) / kGroup];
+            if ((threadIdx.x + i * kThreads) >> 3 >= rows) continue;
+            if (dy_in[i]) dy_next[i] = at<const X8>(dy_at, dy_of[i]);
+            if (x_in[i]) {
+                codes_next[i] = at<const u32x4>(x_at, x_of[i]);
+                e_next[i] = at<const int8_t>(e_at, e_of[i]);
             }
         }
     };

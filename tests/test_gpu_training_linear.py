@@ -224,3 +224,17 @@ def test_refusals(dev):
     w.requires_grad_()
     with pytest.raises(RuntimeError, match="second derivatives"):
         torch.autograd.grad(training.linear_8bit(x, w, b).sum(), w, create_graph=True)
+
+
+@pytest.mark.parametrize("dtype", HALF, ids=str)
+@pytest.mark.parametrize("rows,K", [(5, 16), (70, 48), (300, 80), (70000, 112)])
+def test_an_infinite_weight_stays_infinite(dev, dtype, rows, K):
+    """Short last steps read weights of other columns beside zeros of x."""
+    x = seeded((rows, K), dtype, 1).abs() + 0.5
+    for k in (0, K // 2, K - 1):
+        w = torch.zeros(32, K, dtype=dtype)
+        w[3, k], w[20, k] = math.inf, -math.inf
+        y = training.linear_8bit(x.to(dev), w.to(dev)).cpu()
+        assert (y[:, 3] == math.inf).all() and (y[:, 20] == -math.inf).all()
+        y[:, 3] = y[:, 20] = 0
+        assert (y == 0).all()
