@@ -98,11 +98,7 @@ __device__ __forceinline__ u32x2 quantise(typename Mma<T>::x8 v, int& e) {
         const uint32_t hi = raw[i] & 0x7fff0000u, lo = (raw[i] & 0x7fffu) << 16, more = hi > lo ? hi : lo;
         top = top > more ? top : more;
     }
-#pragma unroll
-    for (int m = 16; m <= 32; m <<= 1) {
-        const uint32_t other = __shfl_xor(top, m);
-        top = top > other ? top : other;
-    }
+    top = max_groups(top);
     const uint32_t bits =
         __float_as_uint(static_cast<float>(__builtin_bit_cast(T, static_cast<unsigned short>(top >> 16))));
     // the largest magnitude is 1.f 2^k; 127 = 1.984375 2^6

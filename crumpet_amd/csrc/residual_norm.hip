@@ -63,11 +63,30 @@ __device__ __forceinline__ void store_row(T* p, const float* v) {
     }
 }
 
+// v plus that of another lane: DPP within 16 lanes, half-wave swaps beyond, which
+// take a few cycles where a shuffle through LDS takes dozens; a row's sums follow
+// one on another.
+template <int kCtrl>
+__device__ __forceinline__ float add_dpp(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float add_halves(float v, bool of_32) {
+    const uint32_t bits = __float_as_uint(v);
+    const auto both = of_32 ? __builtin_amdgcn_permlane32_swap(bits, bits, false, false)
+                            : __builtin_amdgcn_permlane16_swap(bits, bits, false, false);
+    return __uint_as_float(both[0]) + __uint_as_float(both[1]);
+}
+
 // Sum over the G lanes of a row; G = 256 takes a round through LDS.
 template <int G>
 __device__ __forceinline__ float row_sum(float v, float* lds) {
-#pragma unroll
-    for (int m = 1; m < (G < 64 ? G : 64); m <<= 1) v += __shfl_xor(v, m);
+    static_assert(G == 8 || G == 16 || G == 32 || G == 64 || G == 256);
+    v = add_dpp<0xb1>(v);   // lane ^ 1
+    v = add_dpp<0x4e>(v);   // lane ^ 2
+    v = add_dpp<0x141>(v);  // the other four of 8
+    if constexpr (G >= 16) v = add_dpp<0x140>(v);  // the other 8 of 16
+    if constexpr (G >= 32) v = add_halves(v, false);
+    if constexpr (G >= 64) v = add_halves(v, true);
     if constexpr (G == 256) {
         __syncthreads();
         if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
@@ -401,11 +420,13 @@ bool misaligned(std::initializer_list<const void*> ptrs, int64_t C) {
     return false;
 }
 
-// Workgroups of a sample: about 2048 in all, none without a row.
+// Workgroups of a sample: about 1024 in all, none without a row.  Fewer leave
+// compute units idle (768: the gradients of [4, 110592, 48] take 98 us for 84),
+// more write more partial sums (2048: those of [3, 4001, 768] take 62 us for 54).
 uint32_t chunks_of(int64_t samples, int64_t tokens, int64_t C) {
     const int64_t rows = kThreads / shape_of(C).G;
     const int64_t most = (tokens + rows - 1) / rows;
-    return static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(most, (2048 + samples - 1) / samples)));
+    return static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(most, (1024 + samples - 1) / samples)));
 }
 
 }  // namespace

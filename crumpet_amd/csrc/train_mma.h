@@ -174,14 +174,34 @@ __device__ __forceinline__ uint32_t lds_address(const T* p) {
     return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsT*)p)));
 }
 
+// The same lane's values of two groups of 16, in some order: l and l ^ 16, l and
+// l ^ 32; no round trip through LDS.
+struct Two {
+    uint32_t a, b;
+};
+__device__ __forceinline__ Two pair16(uint32_t v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return {r[0], r[1]};
+}
+__device__ __forceinline__ Two pair32(uint32_t v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return {r[0], r[1]};
+}
 // Over the 4 lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48).
 __device__ __forceinline__ float sum_groups(float x) {
-    x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
+    Two t = pair16(__float_as_uint(x));
+    t = pair32(__float_as_uint(__uint_as_float(t.a) + __uint_as_float(t.b)));
+    return __uint_as_float(t.a) + __uint_as_float(t.b);
 }
 __device__ __forceinline__ float max_groups(float x) {
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
+    Two t = pair16(__float_as_uint(x));
+    t = pair32(__float_as_uint(fmaxf(__uint_as_float(t.a), __uint_as_float(t.b))));
+    return fmaxf(__uint_as_float(t.a), __uint_as_float(t.b));
+}
+__device__ __forceinline__ uint32_t max_groups(uint32_t x) {
+    Two t = pair16(x);
+    t = pair32(t.a > t.b ? t.a : t.b);
+    return t.a > t.b ? t.a : t.b;
 }
 
 __device__ __forceinline__ float load_float(const void* p, int32_t dtype, int64_t i) {
