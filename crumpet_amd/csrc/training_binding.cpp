@@ -56,9 +56,12 @@ bool has(const Maybe& t) { return t.has_value() && t->defined(); }
 void* ptr(const Tensor& t) { return t.defined() && t.numel() > 0 ? t.data_ptr() : nullptr; }
 float* floats(const Tensor& t) { return static_cast<float*>(ptr(t)); }
 
+// Without a call where there is nothing to do: a few of them are a microsecond.
+Tensor as_type(const Tensor& t, at::ScalarType type) { return t.scalar_type() == type ? t : t.to(type); }
+
 // Dense and 16-byte aligned.
 Tensor dense(const Tensor& t) {
-    Tensor c = t.contiguous();
+    Tensor c = t.is_contiguous() ? t : t.contiguous();
     return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
 }
 
@@ -68,7 +71,7 @@ Tensor parameter(const Maybe& p, const Tensor& like, at::IntArrayRef shape, cons
     check_device(*p, like, what, name);
     code_of(*p, what, name);
     TORCH_CHECK(p->sizes() == shape, what, ": ", name, " must have shape ", shape, ", got ", p->sizes());
-    return dense(p->to(at::kFloat));
+    return dense(as_type(*p, at::kFloat));
 }
 
 void no_gradient(const Maybe& t, const char* what, const char* name) {
@@ -410,7 +413,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> residual_norm
             floats(a.scale), floats(a.weight), static_cast<float>(eps), ptr(work), stream_of(x)));
     }
     for (int i = 0; i < 5; ++i)
-        if (has(*params[i])) grads[i] = grads[i].to((*params[i])->scalar_type());
+        if (has(*params[i])) grads[i] = as_type(grads[i], (*params[i])->scalar_type());
     return {dx, dy, grads[0], grads[1], grads[2], grads[3], grads[4]};
 }
 
