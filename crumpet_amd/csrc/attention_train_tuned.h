@@ -235,6 +235,8 @@ __device__ __forceinline__ void split(f32x4 v, typename Mma<T>::x4& hi, typename
     }
 }
 
+constexpr float kLargest = 3.40282347e38f;
+
 // The unrolled loops over the tiles are straight-line code, which the compiler
 // would otherwise start all of at once, in registers that it does not have.
 __device__ __forceinline__ void tiles_in_order() {
@@ -347,7 +349,9 @@ __device__ __forceinline__ void build_tiles(f32x4* tile, const AttnArgs& a, int 
                 const int o = in ? other : a.N - 1;
                 float v = bias[kKeysInLanes ? o * a.N + mine : mine * a.N + o];
                 if ((side[o] ^ side[mine]) & kind) v -= 100.0f;
-                v *= per_scale;
+                // fp32's lowest value stays finite: a row of it has equal weights
+                const float folded = fminf(fmaxf(v * per_scale, -kLargest), kLargest);
+                v = fabsf(v) <= kLargest ? folded : v;
                 tile[t][r] = in || kKeysInLanes ? v : -__builtin_inff();
             }
             tiles_in_order();

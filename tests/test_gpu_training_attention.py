@@ -203,6 +203,26 @@ def test_bias_types_and_strides(dev, bias_dtype):
     ref.check({"out": out, "grad_qkv": dqkv, "grad_bias": dbias}, ref.window_attention(qkv, bias, 3, g))
 
 
+@pytest.mark.parametrize("dtype,D", [(torch.float16, 16), (torch.bfloat16, 32), (torch.bfloat16, 64), (torch.float32, 16)],
+                         ids=str)
+@pytest.mark.parametrize("N,shifted", [(40, False), (27, True), (343, True)])
+def test_a_bias_of_the_lowest_value(dev, dtype, D, N, shifted):
+    """fp32's lowest value absorbs a score: a query with nothing else weighs its
+    keys equally, one with a few such keys leaves them out."""
+    qkv, bias, g = _inputs(8, N, 2, D, dtype, seed=N)
+    low = torch.finfo(torch.float32).min
+    bias[0, 1], bias[1, N - 1] = low, low
+    bias[1, 3, ::2] = low
+    where = {}
+    mask = None
+    if shifted:
+        w = round(N ** (1 / 3))
+        where = dict(volume=(2 * w,) * 3, window_size=(w,) * 3, shift_size=(w // 2,) * 3)
+        mask = ref.shift_mask(*where.values())
+    found = _run(dev, qkv, bias, 2, g, **where)
+    ref.check(found, ref.window_attention(qkv, bias, 2, g, torch.zeros(1, N, N) if mask is None else mask))
+
+
 @pytest.mark.parametrize("N", [33, 343])
 def test_mask_views(dev, N):
     qkv, bias, g = _inputs(4, N, 1, 32, torch.bfloat16)
