@@ -32,7 +32,6 @@ constexpr int kThreads = 256;
 constexpr int kGroup = 32;
 constexpr int kNaN = -128;  // exponent byte of a group that is not finite
 
-
 __device__ __forceinline__ float power_of_two(int e) {
     return e == kNaN ? __builtin_nanf("") : __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
@@ -126,11 +125,25 @@ __device__ __forceinline__ u32x2 quantise(typename Mma<T>::x8 v, int& e) {
 }
 
 // Four codes times the group's step: (code + 128) step - 128 step, exact, with
-// one conversion of an unsigned byte each.
+// one conversion of an unsigned byte each.  In the last groups 128 steps
+// overflow fp32 (bf16), and the copy of a number next to the type's largest is
+// rounded up to what the type does not hold (64 2^10, 64 2^122): as an operand
+// it is the largest number.
+template <typename T>
 __device__ __forceinline__ f32x4 values_of(uint32_t codes, float step) {
+    constexpr bool kHalf = std::is_same_v<T, _Float16>;
+    constexpr float kLate = kHalf ? 0x1p10f : 0x1p121f, kMost = kHalf ? 65504.0f : 0x1.fep127f;
     const uint32_t u = codes ^ 0x80808080u;
-    const float less = -128.0f * step;
     f32x4 v;
+    if (step >= kLate) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = (static_cast<float>((u >> (8 * i)) & 0xffu) - 128.0f) * step;
+            v[i] = fminf(fmaxf(x, -kMost), kMost);
+        }
+        return v;
+    }
+    const float less = -128.0f * step;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = __builtin_fmaf(static_cast<float>((u >> (8 * i)) & 0xffu), step, less);
     return v;
@@ -343,7 +356,7 @@ __global__ void __launch_bounds__(kThreads) linear_8bit_rows_kernel(const RowsAr
                 const float step = power_of_two(exps[n][r]);
 #pragma unroll
                 for (int u = 0; u < kEach; ++u) {
-                    const f32x4 x = values_of(codes[n + u][r], step);
+                    const f32x4 x = values_of<T>(codes[n + u][r], step);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) v[u][i] *= act_grad<true>(x[i]);
                 }
@@ -454,7 +467,7 @@ __global__ void __launch_bounds__(kThreads) linear_8bit_weight_kernel(const Weig
             const float step = power_of_two(e_next[i]);
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const f32x4 x = values_of(codes_next[i][w], step);
+                const f32x4 x = values_of<T>(codes_next[i][w], step);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[w >> 1][4 * (w & 1) + e] = static_cast<T>(act<kGelu>(x[e]));
             }
@@ -590,7 +603,8 @@ int check(int32_t dtype, int64_t rows, int64_t K, int64_t n_out, int32_t activat
         return fail(CRUMPET_ERR_UNSUPPORTED, "%s: features in (%lld) and out (%lld) must be multiples of 16 up to 65536",
                     what, (long long)K, (long long)n_out);
     const uint64_t row_blocks = (static_cast<uint64_t>(rows) + 127) / 128;
-    if (!launch_takes(row_blocks * ((std::max(K, n_out) / 16 + 7) / 8) + kNumXcd, kThreads))
+    // blocks of 4 tiles at the least
+    if (!launch_takes(row_blocks * ((std::max(K, n_out) / 16 + 3) / 4) + kNumXcd, kThreads))
         return fail(CRUMPET_ERR_UNSUPPORTED, "%s: too many rows for one launch", what);
     return CRUMPET_OK;
 }

@@ -238,3 +238,28 @@ def test_an_infinite_weight_stays_infinite(dev, dtype, rows, K):
         assert (y[:, 3] == math.inf).all() and (y[:, 20] == -math.inf).all()
         y[:, 3] = y[:, 20] = 0
         assert (y == 0).all()
+
+
+@pytest.mark.parametrize("dtype", HALF, ids=str)
+@pytest.mark.parametrize("activation", ["none", "gelu"])
+def test_the_largest_numbers_stay_finite(dev, dtype, activation):
+    """The copy of the type's largest numbers is rounded up to what the type does
+    not hold (64 steps of the last exponent); as an operand it is the largest."""
+    top = torch.finfo(dtype).max
+    x = torch.zeros(8, 64, dtype=dtype)
+    x[0, 0], x[1, 1], x[2, 40] = top, -top, top / 2
+    x[3, :4] = torch.tensor([top / 4, -top / 3, top / 5, 1.0], dtype=torch.float64).to(dtype)
+    x[4, 32:36] = torch.tensor([top, -top * 0.99, top * 0.3, -top], dtype=torch.float64).to(dtype)
+    kept = ref.eight_bits(x).clamp(-top, top)
+    w = torch.zeros(16, 64, dtype=dtype, device=dev)
+    _, codes, exps = torch.ops.crumpet_ops.linear_8bit_forward(x.to(dev), w, None, int(activation == "gelu"))
+    # a gradient of one row at a time hands the copy back, times 2^-4; of its
+    # GELU the far sides, which are the number itself and 0
+    for r in range(5):
+        g = torch.zeros(8, 16, dtype=dtype, device=dev)
+        g[r, 2] = 2.0 ** -4
+        _, dw, _ = torch.ops.crumpet_ops.linear_8bit_backward(g, codes, exps, w, int(activation == "gelu"), False, True,
+                                                              False)
+        want = kept[r].clamp(min=0) if activation == "gelu" else kept[r]
+        want = torch.where(kept[r].abs() > 100, want, dw[2].cpu().double() * 16) / 16
+        assert torch.equal(dw[2].cpu().double(), want.to(dtype).double())
