@@ -16,6 +16,16 @@
 // transposes come from LDS transpose reads.  The forward pass computes S
 // twice (largest score, then weights) rather than hold it: matrix products
 // are cheap beside the exponentials here.
+//
+// Measured on 1372 windows of 343 tokens and three heads of 16 in fp16: forward
+// 241 us, dq and dbias 308, dk and dv 255, the join of dbias 7.  Issue bounds
+// them, not memory (364 MB in all): VALU 55, 47 and 60% busy, the matrix cores
+// 26, 13 and 19%, with two waves a SIMD, all that the registers of the tiles
+// leave.  Of the forward pass 51 us are the rests of P, which make dbias exact
+// to fp32, 23 the pass for the largest score.  Without a mask tensor a range
+// rebuilds its tiles a few times, which is nothing; with one it does so for
+// every few windows: 128 windows, 64 masks, six heads of 32 in bf16 take 104,
+// 118 and 97 us, about half of it waiting for rows of bias and mask.
 #pragma once
 
 #include <algorithm>

@@ -13,8 +13,17 @@
 // end; act(x) and act(x^) are rounded to the input type once, as operands.
 // Weights are the A operand, rows of x the B operand, so a lane ends with 4
 // neighbouring output features of one row and x passes from memory straight
-// into B fragments: a 32-deep step is one quantisation group, spread over the
-// 4 lane groups.
+// into B fragments: a 32-deep product is one quantisation group, spread over the
+// 4 lane groups.  The weights, which a workgroup's waves share, pass through
+// LDS.
+//
+// Measured, with the GELU, 442368 rows of 192 to 48 in fp16: forward 98 us
+// (300 MB, 3.1 TB/s, VALU 87% busy: the GELU and the codes are 28 instructions a
+// value), dx 103 us (300 MB, VALU 80%), dW and db 107 us (VALU 87%: the GELU
+// again) and 7 for their sums.  Without it the same forward pass takes 84 us.
+// Where products bound it: 27648 rows of 192 to 768 in 32 us (250 TFLOP/s);
+// a step's loads are a step ahead of the products, which is too short a time
+// for more.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -12,6 +12,13 @@
 // values, each rounded once.  Sums over channels and rows are fp32, in a fixed
 // order: each workgroup sums its rows' parameter gradients in registers and
 // writes one row of partial sums, which a second kernel adds up.
+//
+// Measured: [4, 110592, 48], fp32 stream and fp16 branch, layer norm, drop path:
+// forward 46 us (170 MB, 3.7 TB/s), gradients 85 us (340 MB, 4.0 TB/s), their
+// sums 5.  [3, 4001, 768] bf16, rms norms before and after, a gate a sample:
+// forward 22 us (74 MB, 3.3 TB/s), gradients 48 us (111 MB, 2.3 TB/s): 252
+// registers a lane leave two waves to a SIMD, and six to twelve rows to a wave
+// are too few to hide the chain of two norms and their gradients.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -18,7 +18,8 @@ PyTorch for training (torch-ext/crumpet/monai_patch.py:138-142).  Everything
 here runs on HIP devices only and raises elsewhere; sums, softmax statistics
 and norms are fp32 and in a fixed order, so results repeat bit for bit.  The
 calls run on the current stream, can be captured into a graph with their
-backward passes, and have first derivatives only.  Meta and fake tensors are
+backward passes (while no eager autograd graph of the same leaves is alive), and
+have first derivatives only.  Meta and fake tensors are
 supported for tracing.
 """
 
@@ -130,7 +131,8 @@ def window_attention(
     the shifted-window mask of the volume whose windows, in the order of
     ``fused_shift_partition_3d``, ``qkv`` holds (outer batch first), without a
     tensor.  A query whose scores are all -inf gets zeros, and no gradient
-    flows through it.
+    flows through it.  The gradients of the scores are rounded to ``qkv``'s type
+    on their way into those of q and k: in float16 they overflow past 65504.
     """
     ops = _ops(qkv, "window_attention")
     if qkv.dim() != 3:
