@@ -17,10 +17,14 @@
 // its rest (round_and_rest).  dbias is then off by 3e-7 in fp16 and 3 to 9e-7
 // in bf16; with P rounded once it is 2e-5 and 2e-4.
 //
-// Measured on 64 windows of 343 tokens and six heads of 16 in fp32: forward 61
-// us, dq 77, dk and dv 128, dbias 83.  fp32 products (154 TFLOP/s at the most)
-// and the softmax share the issue slots: matrix cores 46, 54, 42 and 36% busy,
-// VALU 50, 48, 34 and 39%.
+// Rows, and the bias before them, are requested a chunk or window ahead: with 16
+// windows of 1000 tokens and six heads of 128 in bf16 the four kernels take 210,
+// 231, 498 and 245 us for 297, 314, 632 and 416.
+//
+// Measured on 64 windows of 343 tokens and six heads of 16 in fp32: forward 60
+// us, dq 74, dk and dv 119, dbias 79.  fp32 products (154 TFLOP/s at the most)
+// and the softmax share the issue slots: matrix cores 44, 54, 43 and 40% busy,
+// VALU 52, 51, 36 and 46%.
 #pragma once
 
 #include <algorithm>
@@ -77,16 +81,38 @@ struct Terms {
         if (a.mode == kTensorMask) mask_at = static_cast<int64_t>(b % a.mask_batch) * a.mask_sb;
         if (a.mode == kRegionMask) seam = seams(a.region, b);
     }
-    // Scores of query q and keys k .. k + 3; keys past N are -inf.  cls: the
-    // region classes of the keys.
-    __device__ __forceinline__ f32x4 of_query(const AttnArgs& a, f32x4 qk, int q, int k, uint32_t cq,
+    // The bias of query q and keys k .. k + 3, and of queries q .. q + 3 and key
+    // k; read before a chunk's scores and before the next chunk's rows are
+    // requested, since loads come back in order.
+    __device__ __forceinline__ f32x4 of_row(const AttnArgs& a, int q, int k) const {
+        const float* at = bias + static_cast<uint32_t>(q * a.N + k);  // N^2 is below 2^29
+        f32x4 v = {};
+        if (k + 4 <= a.N) {
+            const Four<float> b = *reinterpret_cast<const Four<float>*>(at);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = b.v[r];
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (k + r < a.N) v[r] = at[r];
+        }
+        return v;
+    }
+    __device__ __forceinline__ f32x4 of_column(const AttnArgs& a, int q, int k) const {
+        f32x4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = bias[static_cast<uint32_t>((q + r < a.N ? q + r : a.N - 1) * a.N + k)];
+        return v;
+    }
+    // Scores of query q and keys k .. k + 3; keys past N are -inf.  b: their bias,
+    // cls: the region classes of the keys.
+    __device__ __forceinline__ f32x4 of_query(const AttnArgs& a, f32x4 qk, f32x4 b, int q, int k, uint32_t cq,
                                               const uint32_t* cls) const {
         const int64_t at = static_cast<int64_t>(q) * a.N + k;
         f32x4 s;
         if (k + 4 <= a.N) {
-            const Four<float> b = *reinterpret_cast<const Four<float>*>(bias + at);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[r] = __builtin_fmaf(qk[r], a.scale, b.v[r]);
+            for (int r = 0; r < 4; ++r) s[r] = __builtin_fmaf(qk[r], a.scale, b[r]);
             if (a.mode == kTensorMask) {
                 if (a.mask_dtype == CRUMPET_DTYPE_F32) add<float>(s, at);
                 else if (a.mask_dtype == CRUMPET_DTYPE_F16) add<_Float16>(s, at);
@@ -97,7 +123,7 @@ struct Terms {
             for (int r = 0; r < 4; ++r) {
                 s[r] = -__builtin_inff();
                 if (k + r >= a.N) continue;
-                s[r] = __builtin_fmaf(qk[r], a.scale, bias[at + r]);
+                s[r] = __builtin_fmaf(qk[r], a.scale, b[r]);
                 if (a.mode == kTensorMask) s[r] += load_float(mask, a.mask_dtype, mask_at + at + r);
             }
         }
@@ -108,13 +134,13 @@ struct Terms {
         return s;
     }
     // Scores of queries q .. q + 3 and key k; rows past N are anything.
-    __device__ __forceinline__ f32x4 of_key(const AttnArgs& a, f32x4 qk, int q, int k, const uint32_t* cls,
+    __device__ __forceinline__ f32x4 of_key(const AttnArgs& a, f32x4 qk, f32x4 b, int q, int k, const uint32_t* cls,
                                             uint32_t ck) const {
         f32x4 s;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int64_t at = static_cast<int64_t>(q + r < a.N ? q + r : a.N - 1) * a.N + k;
-            s[r] = __builtin_fmaf(qk[r], a.scale, bias[at]);
+            s[r] = __builtin_fmaf(qk[r], a.scale, b[r]);
             if (a.mode == kTensorMask) s[r] += load_float(mask, a.mask_dtype, mask_at + at);
             if (seam) s[r] -= ck != cls[r] ? 100.0f : 0.0f;
         }
@@ -136,17 +162,29 @@ __device__ __forceinline__ const T* token_row(const AttnArgs& a, uint32_t b, int
            (static_cast<int64_t>(which) * a.H + h) * D;
 }
 
-// Rows row0 .. row0 + kRows - 1 (those past N repeat the last one) into LDS.
+// Rows row0 .. row0 + kRows - 1 (those past N repeat the last one) on their way
+// into LDS: requested a chunk ahead, stored when the chunk before is done.
 template <typename T, int D>
-__device__ __forceinline__ void stage(T* lds, const T* first, int64_t stride, int row0, int N) {
+struct Staged {
     typedef Tile<T, D> L;
-    constexpr int kPieces = D / 4;
-    for (int i = threadIdx.x; i < L::kRows * kPieces; i += kThreads) {
-        const int r = i / kPieces, c = i % kPieces * 4;
-        const int row = row0 + r < N ? row0 + r : N - 1;
-        *reinterpret_cast<typename Mma<T>::x4*>(lds + r * L::kLd + c) = load4<T>(first + row * stride + c);
+    static constexpr int kPieces = D / 4, kEach = L::kRows * kPieces / kThreads;
+    static_assert(kEach * kThreads == L::kRows * kPieces);
+    typename Mma<T>::x4 v[kEach];
+    __device__ __forceinline__ void fetch(const T* first, int64_t stride, int row0, int N) {
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+            const int i = threadIdx.x + u * kThreads, row = row0 + i / kPieces;
+            v[u] = load4<T>(first + (row < N ? row : N - 1) * stride + i % kPieces * 4);
+        }
     }
-}
+    __device__ __forceinline__ void store(T* lds) const {
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+            const int i = threadIdx.x + u * kThreads;
+            *reinterpret_cast<typename Mma<T>::x4*>(lds + i / kPieces * L::kLd + i % kPieces * 4) = v[u];
+        }
+    }
+};
 
 template <typename T, int D>
 struct Rows {  // a lane's fragments of 16 rows: row col, columns 16 s + 4 g ..
@@ -207,20 +245,29 @@ __global__ void __launch_bounds__(kThreads) attn_forward_kernel(const AttnArgs a
     qr.load(token_row<T>(a, b, q, 0, h, D), g);
     f32x4 acc[L::kSlices] = {};
     float top = -__builtin_inff(), total = 0.0f;
+    const T *k_at = token_row<T>(a, b, 0, 1, h, D), *v_at = token_row<T>(a, b, 0, 2, h, D);
+    Staged<T, D> ks, vs;
+    ks.fetch(k_at, a.st, 0, a.N), vs.fetch(v_at, a.st, 0, a.N);
     for (int k0 = 0; k0 < a.N; k0 += L::kRows) {
         __syncthreads();
-        stage<T, D>(k_lds, token_row<T>(a, b, 0, 1, h, D), a.st, k0, a.N);
-        stage<T, D>(v_lds, token_row<T>(a, b, 0, 2, h, D), a.st, k0, a.N);
+        ks.store(k_lds), vs.store(v_lds);
         if (threadIdx.x < L::kRows)
             cls[threadIdx.x] = terms.seam && k0 + static_cast<int>(threadIdx.x) < a.N
                                    ? token_class(a.region, terms.seam, k0 + threadIdx.x) : 0;
         __syncthreads();
+        f32x4 bias[L::kRows / 16];
+#pragma unroll
+        for (int t = 0; t < L::kRows / 16; ++t) bias[t] = terms.of_row(a, q, k0 + 16 * t + 4 * g);
+        if (k0 + L::kRows < a.N) {
+            ks.fetch(k_at, a.st, k0 + L::kRows, a.N);
+            vs.fetch(v_at, a.st, k0 + L::kRows, a.N);
+        }
         f32x4 s[L::kRows / 16];
         float high = top;
 #pragma unroll
         for (int t = 0; t < L::kRows / 16; ++t) {
             const int i = 16 * t + 4 * g;
-            s[t] = terms.of_query(a, product<T, D>(k_lds, 16 * t, qr, col, g), q, k0 + i, cq, cls + i);
+            s[t] = terms.of_query(a, product<T, D>(k_lds, 16 * t, qr, col, g), bias[t], q, k0 + i, cq, cls + i);
 #pragma unroll
             for (int r = 0; r < 4; ++r) high = fmaxf(high, s[t][r]);
         }
@@ -314,18 +361,34 @@ __global__ void __launch_bounds__(kThreads) attn_grad_q_kernel(const AttnArgs a,
     const float delta = row_delta<T, D>(a, at, go, g);
     const float top = a.row_max[row], inv = a.row_inv[row];
     f32x4 acc[L::kSlices] = {};
+    const T *k_at = token_row<T>(a, b, 0, 1, h, D), *v_at = token_row<T>(a, b, 0, 2, h, D);
+    Staged<T, D> ks, vs;
+    // Not in fp32: its rows' registers cost a wave (64 windows of 343 tokens, six
+    // heads of 16: 80 us for 72).  fp16, heads of 64: 95 us for 128.
+    constexpr bool kAhead = sizeof(T) == 2;
+    if constexpr (kAhead) ks.fetch(k_at, a.st, 0, a.N), vs.fetch(v_at, a.st, 0, a.N);
     for (int k0 = 0; k0 < a.N; k0 += L::kRows) {
+        if constexpr (!kAhead) ks.fetch(k_at, a.st, k0, a.N), vs.fetch(v_at, a.st, k0, a.N);
         __syncthreads();
-        stage<T, D>(k_lds, token_row<T>(a, b, 0, 1, h, D), a.st, k0, a.N);
-        stage<T, D>(v_lds, token_row<T>(a, b, 0, 2, h, D), a.st, k0, a.N);
+        ks.store(k_lds), vs.store(v_lds);
         if (threadIdx.x < L::kRows)
             cls[threadIdx.x] = terms.seam && k0 + static_cast<int>(threadIdx.x) < a.N
                                    ? token_class(a.region, terms.seam, k0 + threadIdx.x) : 0;
         __syncthreads();
+        f32x4 bias[L::kRows / 16];
+        if constexpr (kAhead) {
+#pragma unroll
+            for (int t = 0; t < L::kRows / 16; ++t) bias[t] = terms.of_row(a, q, k0 + 16 * t + 4 * g);
+            if (k0 + L::kRows < a.N) {
+                ks.fetch(k_at, a.st, k0 + L::kRows, a.N);
+                vs.fetch(v_at, a.st, k0 + L::kRows, a.N);
+            }
+        }
 #pragma unroll
         for (int t = 0; t < L::kRows / 16; ++t) {
             const int i = 16 * t + 4 * g;
-            f32x4 s = terms.of_query(a, product<T, D>(k_lds, 16 * t, qr, col, g), q, k0 + i, cq, cls + i);
+            if constexpr (!kAhead) bias[t] = terms.of_row(a, q, k0 + i);
+            f32x4 s = terms.of_query(a, product<T, D>(k_lds, 16 * t, qr, col, g), bias[t], q, k0 + i, cq, cls + i);
             const f32x4 dp = product<T, D>(v_lds, 16 * t, go, col, g);
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[r] = k0 + i + r < a.N ? weight(s[r], top) * inv * (dp[r] - delta) : 0.0f;
@@ -361,23 +424,35 @@ __global__ void __launch_bounds__(kThreads) attn_grad_kv_kernel(const AttnArgs a
     kr.load(token_row<T>(a, b, k, 1, h, D), g);
     vr.load(token_row<T>(a, b, k, 2, h, D), g);
     f32x4 dk[L::kSlices] = {}, dv[L::kSlices] = {};
-    for (int q0 = 0; q0 < a.N; q0 += L::kRows) {
-        __syncthreads();
-        stage<T, D>(q_lds, token_row<T>(a, b, 0, 0, h, D), a.st, q0, a.N);
-        stage<T, D>(o_lds, go, static_cast<int64_t>(a.H) * D, q0, a.N);
+    const T* q_at = token_row<T>(a, b, 0, 0, h, D);
+    Staged<T, D> qs, os;
+    float top_next = 0.0f, inv_next = 0.0f, delta_next = 0.0f;
+    const auto fetch = [&](int q0) {
+        qs.fetch(q_at, a.st, q0, a.N), os.fetch(go, static_cast<int64_t>(a.H) * D, q0, a.N);
         if (threadIdx.x < L::kRows) {
             const int q = q0 + static_cast<int>(threadIdx.x);
-            const bool in = q < a.N;
-            top[threadIdx.x] = in ? a.row_max[first + q] : 0.0f;
-            inv[threadIdx.x] = in ? a.row_inv[first + q] : 0.0f;
-            delta[threadIdx.x] = in ? a.delta[first + q] : 0.0f;
-            cls[threadIdx.x] = in && terms.seam ? token_class(a.region, terms.seam, q) : 0;
+            const int64_t row = first + (q < a.N ? q : a.N - 1);
+            top_next = a.row_max[row], inv_next = a.row_inv[row], delta_next = a.delta[row];
+        }
+    };
+    fetch(0);
+    for (int q0 = 0; q0 < a.N; q0 += L::kRows) {
+        __syncthreads();
+        qs.store(q_lds), os.store(o_lds);
+        if (threadIdx.x < L::kRows) {
+            const int q = q0 + static_cast<int>(threadIdx.x);
+            top[threadIdx.x] = top_next, inv[threadIdx.x] = inv_next, delta[threadIdx.x] = delta_next;
+            cls[threadIdx.x] = q < a.N && terms.seam ? token_class(a.region, terms.seam, q) : 0;
         }
         __syncthreads();
+        f32x4 bias[L::kRows / 16];
+#pragma unroll
+        for (int t = 0; t < L::kRows / 16; ++t) bias[t] = terms.of_column(a, q0 + 16 * t + 4 * g, k);
+        if (q0 + L::kRows < a.N) fetch(q0 + L::kRows);
 #pragma unroll
         for (int t = 0; t < L::kRows / 16; ++t) {
             const int first = 16 * t + 4 * g;
-            f32x4 p = terms.of_key(a, product<T, D>(q_lds, 16 * t, kr, col, g), q0 + first, k, cls + first, ck);
+            f32x4 p = terms.of_key(a, product<T, D>(q_lds, 16 * t, kr, col, g), bias[t], q0 + first, k, cls + first, ck);
             f32x4 ds = product<T, D>(o_lds, 16 * t, vr, col, g);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -416,26 +491,39 @@ __global__ void __launch_bounds__(kThreads) attn_grad_bias_kernel(const AttnArgs
     const uint32_t chunk = id / a.H;
     const int q = q0 < a.N ? q0 : a.N - 1;
     f32x4 acc[L::kRows / 16] = {};
+    Staged<T, D> ks, vs;
+    Rows<T, D> qn, gn;
+    float delta_next = 0.0f, top_next = 0.0f, inv_next = 0.0f;
+    const auto fetch = [&](uint32_t b) {
+        const int64_t at = (static_cast<int64_t>(b) * a.N + q) * a.H + h;
+        const int64_t row = (static_cast<int64_t>(b) * a.H + h) * a.N + q;
+        ks.fetch(token_row<T>(a, b, 0, 1, h, D), a.st, k0, a.N);
+        vs.fetch(token_row<T>(a, b, 0, 2, h, D), a.st, k0, a.N);
+        qn.load(token_row<T>(a, b, q, 0, h, D), g);
+        gn.load(static_cast<const T*>(a.grad_out) + at * D, g);
+        delta_next = a.delta[row], top_next = a.row_max[row], inv_next = a.row_inv[row];
+    };
+    if (chunk < a.B) fetch(chunk);
+    // the same for every window
+    f32x4 bias[L::kRows / 16];
+#pragma unroll
+    for (int t = 0; t < L::kRows / 16; ++t) bias[t] = Terms(a, 0, h).of_row(a, q, k0 + 16 * t + 4 * g);
     for (uint32_t b = chunk; b < a.B; b += a.chunks) {
         const Terms terms(a, b, h);
         const uint32_t cq = terms.seam ? token_class(a.region, terms.seam, q) : 0;
-        const int64_t at = (static_cast<int64_t>(b) * a.N + q) * a.H + h;
-        const int64_t row = (static_cast<int64_t>(b) * a.H + h) * a.N + q;
-        Rows<T, D> qr, go;
-        qr.load(token_row<T>(a, b, q, 0, h, D), g);
-        go.load(static_cast<const T*>(a.grad_out) + at * D, g);
-        const float delta = a.delta[row], top = a.row_max[row], inv = a.row_inv[row];
+        const Rows<T, D> qr = qn, go = gn;
+        const float delta = delta_next, top = top_next, inv = inv_next;
         __syncthreads();
-        stage<T, D>(k_lds, token_row<T>(a, b, 0, 1, h, D), a.st, k0, a.N);
-        stage<T, D>(v_lds, token_row<T>(a, b, 0, 2, h, D), a.st, k0, a.N);
+        ks.store(k_lds), vs.store(v_lds);
         if (threadIdx.x < L::kRows)
             cls[threadIdx.x] = terms.seam && k0 + static_cast<int>(threadIdx.x) < a.N
                                    ? token_class(a.region, terms.seam, k0 + threadIdx.x) : 0;
         __syncthreads();
+        if (a.B - b > a.chunks) fetch(b + a.chunks);
 #pragma unroll
         for (int t = 0; t < L::kRows / 16; ++t) {
             const int i = 16 * t + 4 * g;
-            const f32x4 s = terms.of_query(a, product<T, D>(k_lds, 16 * t, qr, col, g), q, k0 + i, cq, cls + i);
+            const f32x4 s = terms.of_query(a, product<T, D>(k_lds, 16 * t, qr, col, g), bias[t], q, k0 + i, cq, cls + i);
             const f32x4 dp = product<T, D>(v_lds, 16 * t, go, col, g);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
