@@ -37,7 +37,11 @@ int64_t rounded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 // The bias-stationary kernels: 16-bit types, head dims 16 and 32, up to 512
 // tokens.  Without a mask tensor they fold the scale into the bias, which
 // needs a scale whose inverse is an ordinary number.  Offsets in a window's rows
-// take 32 bits there.
+// take 32 bits there.  Forward and gradients, against the general kernels: 1372
+// windows of 343 tokens, three heads of 16, 794 us for 1753; 1000 of 27, six heads
+// of 16, 68 for 122; 4 of 216, 24 heads of 16, 51 for 61; one of 27 and one head
+// 13 for 17; 64 masks of 343, six heads of 32, 221 for 431.  (Of small calls the
+// forward pass alone is 1 to 5 us slower, but both passes share the statistics.)
 bool use_tuned(const AttnArgs& a, int32_t dtype, int64_t D) {
     if (a.st < 0 || a.st >= int64_t(1) << 21 || a.H > 4096) return false;
     const bool folds = a.scale >= 0x1p-20f && a.scale <= 0x1p20f;
