@@ -501,7 +501,8 @@ CRUMPET_API int crumpet_residual_norm_backward(
  * [rows, K] and exponents [rows, ceil(K / 32)] (both or neither) receive x in 8
  * bits: codes times 2^e for every 32 columns of a row, e the least integer >=
  * -126 with 127 2^e >= their largest magnitude; -128 marks a group that is
- * not finite, kept as NaN.
+ * not finite, kept as NaN.  A number next to the type's largest is rounded up
+ * past it; as an operand of the backward pass it is the largest.
  *
  * The backward pass: grad_x = (grad_y weight) act'(x^), grad_weight = grad_y^T
  * act(x^), grad_bias = sum of grad_y, each optional, with x^ the 8-bit copy.
