@@ -14,14 +14,15 @@
 // writes one row of partial sums, which a second kernel adds up.
 //
 // Measured: [4, 110592, 48], fp32 stream and fp16 branch, layer norm, drop path:
-// forward 46 us (170 MB, 3.7 TB/s), gradients 85 us (340 MB, 4.0 TB/s), their
+// forward 46 us (255 MB, 5.5 TB/s), gradients 78 us (382 MB, 4.9 TB/s), their
 // sums 5.  [3, 4001, 768] bf16, rms norms before and after, a gate a sample:
-// forward 22 us (74 MB, 3.3 TB/s), gradients 48 us (111 MB, 2.3 TB/s): 252
+// forward 18 us (74 MB, 4.1 TB/s), gradients 48 us (111 MB, 2.3 TB/s): 252
 // registers a lane leave two waves to a SIMD, and six to twelve rows to a wave
 // are too few to hide the chain of two norms and their gradients.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "crumpet_common.h"
 #include "crumpet_hip.h"
@@ -130,6 +131,33 @@ struct Lane {
             }
         }
     }
+    // The same in two steps: a row on its way, and its numbers.
+    template <typename T>
+    struct Ahead {
+        typedef T Many __attribute__((ext_vector_type(E == 1 ? 2 : E)));
+        std::conditional_t<E == 1, T, Many> v[NV];
+    };
+    template <typename T>
+    __device__ __forceinline__ void fetch(const T* row, Ahead<T>& to) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (in[i]) to.v[i] = *reinterpret_cast<const std::remove_reference_t<decltype(to.v[i])>*>(row + at[i]);
+    }
+    template <typename T>
+    __device__ __forceinline__ void widen(const Ahead<T>& from, float* v) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                T one;
+                if constexpr (E == 1)
+                    one = from.v[i];
+                else
+                    one = from.v[i][e];
+                v[i * E + e] = in[i] ? static_cast<float>(one) : 0.0f;
+            }
+        }
+    }
     template <typename T>
     __device__ __forceinline__ void store(T* row, const float* v) const {
 #pragma unroll
@@ -193,11 +221,22 @@ __global__ void __launch_bounds__(kThreads) residual_norm_kernel(const NormArgs 
     for (int i = 0; i < kN; ++i) kg[i] *= k;
     const uint32_t step = a.chunks * kRows;
     // every lane of a workgroup-wide row takes part in each round
-    for (uint32_t t = chunk * kRows + threadIdx.x / G; t < a.T; t += step) {
+    typename Lane<E, NV, G>::template Ahead<Tx> x_next = {};
+    typename Lane<E, NV, G>::template Ahead<Ty> y_next = {};
+    const auto fetch = [&](uint32_t t) {
+        const int64_t row = (static_cast<int64_t>(sample) * a.T + t) * a.C;
+        lane.fetch(static_cast<const Tx*>(a.x) + row, x_next);
+        lane.fetch(static_cast<const Ty*>(a.y) + row, y_next);
+    };
+    // rows a round ahead: [3, 4001, 768] bf16 18 us for 22
+    uint32_t t = chunk * kRows + threadIdx.x / G;
+    if (t < a.T) fetch(t);
+    for (; t < a.T; t += step) {
         const int64_t row = (static_cast<int64_t>(sample) * a.T + t) * a.C;
         float x[kN], y[kN];
-        lane.load(static_cast<const Tx*>(a.x) + row, x);
-        lane.load(static_cast<const Ty*>(a.y) + row, y);
+        lane.widen(x_next, x);
+        lane.widen(y_next, y);
+        if (t + step < a.T) fetch(t + step);
         if (a.post) {
             float pw[kN], pb[kN];
             lane.load(a.pw, pw, 1.0f);
@@ -228,13 +267,36 @@ __global__ void __launch_bounds__(kThreads) residual_norm_grad_kernel(const Norm
     const float* gate = a.gate != nullptr ? a.gate + static_cast<int64_t>(sample) * a.gate_stride : nullptr;
     float sums[kMine][kN] = {};
     const uint32_t step = a.chunks * kRows;
-    for (uint32_t t = chunk * kRows + threadIdx.x / G; t < a.T; t += step) {
+    // Rows a round ahead where a lane holds one vector ([4, 110592, 48], fp32 and
+    // fp16: 78 us for 85); two fill the registers ([3, 4001, 768] bf16 with both
+    // norms: 57 for 48).
+    constexpr bool kAhead = kN <= 8;
+    typename Lane<E, NV, G>::template Ahead<Tx> x_next = {}, sum_next = {};
+    typename Lane<E, NV, G>::template Ahead<Ty> y_next = {}, out_next = {};
+    const auto fetch = [&](uint32_t t) {
+        const int64_t row = (static_cast<int64_t>(sample) * a.T + t) * a.C;
+        lane.fetch(static_cast<const Tx*>(a.x) + row, x_next);
+        lane.fetch(static_cast<const Ty*>(a.y) + row, y_next);
+        if (a.gout != nullptr) lane.fetch(static_cast<const Ty*>(a.gout) + row, out_next);
+        if (a.gsum != nullptr) lane.fetch(static_cast<const Tx*>(a.gsum) + row, sum_next);
+    };
+    uint32_t t = chunk * kRows + threadIdx.x / G;
+    if (kAhead && t < a.T) fetch(t);
+    for (; t < a.T; t += step) {
         const int64_t row = (static_cast<int64_t>(sample) * a.T + t) * a.C;
         float n[kN], y[kN], gx[kN], other[kN], yr = 0.0f;
-        lane.load(static_cast<const Tx*>(a.x) + row, n);
-        lane.load(static_cast<const Ty*>(a.y) + row, y);
-        lane.load(a.gout != nullptr ? static_cast<const Ty*>(a.gout) + row : nullptr, gx);
-        lane.load(a.gsum != nullptr ? static_cast<const Tx*>(a.gsum) + row : nullptr, other);
+        if constexpr (kAhead) {
+            lane.widen(x_next, n);
+            lane.widen(y_next, y);
+            lane.widen(out_next, gx);
+            lane.widen(sum_next, other);
+            if (t + step < a.T) fetch(t + step);
+        } else {
+            lane.load(static_cast<const Tx*>(a.x) + row, n);
+            lane.load(static_cast<const Ty*>(a.y) + row, y);
+            lane.load(a.gout != nullptr ? static_cast<const Ty*>(a.gout) + row : nullptr, gx);
+            lane.load(a.gsum != nullptr ? static_cast<const Tx*>(a.gsum) + row : nullptr, other);
+        }
         if constexpr (kPost) yr = lane.normalise(y, a.C, a.rms, a.post_eps, lds);
         // y' = y p + b, made again where it is needed again
         const auto branch = [&](float* u) {
