@@ -126,8 +126,8 @@ def window_attention(
     ``head_dim ** -0.5`` by default.  ``bias`` may have any of the types and
     receives its gradient in its own, summed in fp32.
 
-    ``mask`` is added to the scores, window b reads ``mask[b mod masks]``; it
-    has no gradient.  Or ``volume``, ``window_size`` and ``shift_size`` give
+    ``mask`` is added to the scores, window b reads ``mask[b mod masks]`` (the
+    windows are a multiple of the masks); it has no gradient.  Or ``volume``, ``window_size`` and ``shift_size`` give
     the shifted-window mask of the volume whose windows, in the order of
     ``fused_shift_partition_3d``, ``qkv`` holds (outer batch first), without a
     tensor.  A query whose scores are all -inf gets zeros, and no gradient
