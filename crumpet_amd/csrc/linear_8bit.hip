@@ -19,8 +19,8 @@
 //
 // Measured, with the GELU, 442368 rows of 192 to 48 in fp16: forward 98 us
 // (300 MB, 3.1 TB/s, VALU 87% busy: the GELU and the codes are 28 instructions a
-// value), dx 103 us (300 MB, VALU 80%), dW and db 107 us (VALU 87%: the GELU
-// again) and 7 for their sums.  Without it the same forward pass takes 84 us.
+// value), dx 103 us (300 MB, VALU 80%), dW and db 98 us (VALU 95%: the GELU
+// again) and 7 for their sums, which one chunk of rows does without.  Without it the same forward pass takes 84 us.
 // Where products bound it: 27648 rows of 192 to 768 in 32 us (250 TFLOP/s);
 // a step's loads are a step ahead of the products, which is too short a time
 // for more.
@@ -401,7 +401,8 @@ struct WeightArgs {
     const void* dy;          // [rows, n_out]
     const int8_t* codes;     // [rows, K]
     const int8_t* exps;
-    float* partial;          // [chunks, n_out K + n_out]
+    float* partial;          // [chunks, n_out K + n_out], or null with one chunk:
+    void *dw, *db;           // the results, each or null
     int64_t rows, per;       // rows of a chunk
     int32_t K, n_out;
     uint32_t kblocks, nblocks;
@@ -509,21 +510,31 @@ __global__ void __launch_bounds__(kThreads) linear_8bit_weight_kernel(const Weig
             }
         }
     }
-    float* to = a.partial + chunk * (static_cast<int64_t>(a.n_out) * a.K + a.n_out);
+    const auto put = [&](auto* weights, auto* sums) {
+        typedef std::remove_reference_t<decltype(*sums)> To;
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
+        for (int n = 0; n < 4; ++n) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int f = n0 + 16 * n + 4 * g + r;
-            if (f >= a.n_out) continue;
+            for (int r = 0; r < 4; ++r) {
+                const int f = n0 + 16 * n + 4 * g + r;
+                if (f >= a.n_out) continue;
+                if (weights != nullptr) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int k = k0 + 32 * wave + 16 * t + col;
-                if (k < a.K) to[static_cast<int64_t>(f) * a.K + k] = acc[n][t][r];
+                    for (int t = 0; t < 2; ++t) {
+                        const int k = k0 + 32 * wave + 16 * t + col;
+                        if (k < a.K) weights[static_cast<int64_t>(f) * a.K + k] = static_cast<To>(acc[n][t][r]);
+                    }
+                }
+                if (sum_dy && col == 0 && sums != nullptr) sums[f] = static_cast<To>(db[n][r]);
             }
-            if (sum_dy && col == 0) to[static_cast<int64_t>(a.n_out) * a.K + f] = db[n][r];
         }
+    };
+    if (a.partial == nullptr) {
+        put(static_cast<T*>(a.dw), static_cast<T*>(a.db));
+        return;
     }
+    float* to = a.partial + chunk * (static_cast<int64_t>(a.n_out) * a.K + a.n_out);
+    put(to, to + static_cast<int64_t>(a.n_out) * a.K);
 }
 
 // Sums of the chunks: 32 numbers by 8 groups of chunks per workgroup, each group
@@ -645,13 +656,15 @@ int backward(void* dx, void* dw, void* db, const void* dy, const int8_t* codes, 
     const Split p = split_rows(rows, K, n_out);
     WeightArgs a = {};
     a.dy = dy, a.codes = codes, a.exps = exps, a.rows = rows, a.per = p.per, a.K = k, a.n_out = n;
-    a.partial = reinterpret_cast<float*>(workspace + (K * n_out * 2 + 255) / 256 * 256);
+    a.dw = dw, a.db = db;
+    if (p.chunks > 1) a.partial = reinterpret_cast<float*>(workspace + (K * n_out * 2 + 255) / 256 * 256);
     a.kblocks = p.kblocks, a.nblocks = p.nblocks;
     const uint32_t grid = static_cast<uint32_t>(p.chunks) * p.kblocks * p.nblocks;
     if (activation)
         linear_8bit_weight_kernel<T, true><<<grid, kThreads, 0, s>>>(a);
     else
         linear_8bit_weight_kernel<T, false><<<grid, kThreads, 0, s>>>(a);
+    if (p.chunks == 1) return check_launch("linear_8bit_backward");
     const int64_t all = n_out * K + n_out;
     linear_8bit_join_kernel<T><<<static_cast<uint32_t>((all + 31) / 32), kThreads, 0, s>>>(
         static_cast<T*>(dw), static_cast<T*>(db), a.partial, n_out * K, all, p.chunks);
@@ -687,7 +700,8 @@ extern "C" int crumpet_linear_8bit(void* y, int8_t* codes, int8_t* exponents, co
 extern "C" int64_t crumpet_linear_8bit_workspace(int64_t rows, int64_t K, int64_t n_out) {
     if (train::check(CRUMPET_DTYPE_F16, rows, K, n_out, 0, "linear_8bit_workspace") != CRUMPET_OK) return -1;
     if (rows == 0) return 0;
-    return (K * n_out * 2 + 255) / 256 * 256 + split_rows(rows, K, n_out).chunks * (n_out * K + n_out) * 4;
+    const int64_t chunks = split_rows(rows, K, n_out).chunks;
+    return (K * n_out * 2 + 255) / 256 * 256 + (chunks > 1 ? chunks * (n_out * K + n_out) * 4 : 0);
 }
 
 extern "C" int crumpet_linear_8bit_backward(void* grad_x, void* grad_weight, void* grad_bias, const void* grad_y,

@@ -263,3 +263,20 @@ def test_the_largest_numbers_stay_finite(dev, dtype, activation):
         want = kept[r].clamp(min=0) if activation == "gelu" else kept[r]
         want = torch.where(kept[r].abs() > 100, want, dw[2].cpu().double() * 16) / 16
         assert torch.equal(dw[2].cpu().double(), want.to(dtype).double())
+
+
+@pytest.mark.parametrize("rows", [64, 700])
+@pytest.mark.parametrize("wanted", [(0,), (1,), (2,), (0, 2), (1, 2)], ids=str)
+def test_some_of_the_gradients(dev, rows, wanted):
+    """One chunk of rows, whose sums are the results, and several."""
+    leaves = [t.to(dev) for t in _inputs(rows, 48, 80, torch.float16)]
+    g = leaves.pop()
+
+    def run(which):
+        x, w, b = (t.clone().requires_grad_(i in which) for i, t in enumerate(leaves))
+        y = training.linear_8bit(x, w, b, activation="gelu")
+        return torch.autograd.grad(y, [t for i, t in enumerate((x, w, b)) if i in which], g)
+
+    whole = run((0, 1, 2))
+    for i, d in zip(wanted, run(wanted), strict=True):
+        assert torch.equal(d, whole[i])
