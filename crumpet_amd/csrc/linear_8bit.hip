@@ -700,8 +700,7 @@ extern "C" int crumpet_linear_8bit(void* y, int8_t* codes, int8_t* exponents, co
 extern "C" int64_t crumpet_linear_8bit_workspace(int64_t rows, int64_t K, int64_t n_out) {
     if (train::check(CRUMPET_DTYPE_F16, rows, K, n_out, 0, "linear_8bit_workspace") != CRUMPET_OK) return -1;
     if (rows == 0) return 0;
-    const int64_t chunks = split_rows(rows, K, n_out).chunks;
-    return (K * n_out * 2 + 255) / 256 * 256 + (chunks > 1 ? chunks * (n_out * K + n_out) * 4 : 0);
+    return (K * n_out * 2 + 255) / 256 * 256 + split_rows(rows, K, n_out).chunks * (n_out * K + n_out) * 4;
 }
 
 extern "C" int crumpet_linear_8bit_backward(void* grad_x, void* grad_weight, void* grad_bias, const void* grad_y,
